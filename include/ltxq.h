@@ -16,6 +16,7 @@
  *                              transformer.py:387,484 text-CA gate-then-add)
  *   ltxq_head_gate       <- LTX_2_MLX/model/transformer/attention.py:559-601
  *   ltxq_qk_norm_rope    <- attention.py:320-329, 580-587 + rope.py:53-90
+ *   ltxq_rotary          <- rope.py:53-90 and its interleaved form, from positions
  *   ltxq_attention       <- mx.fast.scaled_dot_product_attention in
  *                           attention.py:170-302 (kernels/steel_attention.py)
  *   ltxq_quantize        <- mx.quantize at loader/transformer_cache.py:1255
@@ -60,7 +61,7 @@ enum {
 
 enum { LTXQ_BF16 = 0, LTXQ_F32 = 1 };                              /* element dtypes */
 enum { LTXQ_NORM_NONE = 0, LTXQ_NORM_RMS = 1, LTXQ_NORM_LAYER = 2 }; /* prologue norm */
-enum { LTXQ_AFFINE = 0, LTXQ_MXFP8 = 1 };                           /* quantization mode */
+enum { LTXQ_AFFINE = 0, LTXQ_MXFP8 = 1, LTXQ_MXFP4 = 2, LTXQ_NVFP4 = 3 }; /* quantization mode */
 enum { LTXQ_LAYOUT_STD = 0, LTXQ_LAYOUT_PRETRANSPOSED = 1 };        /* packed-weight layout */
 enum {
   LTXQ_EPI_NONE = 0,           /* out = bf16(bf16(acc) + bias)                        */
@@ -97,32 +98,51 @@ enum {
  * DEQUANT kernels.  The MX modes need workspace for the split
  * activations (ltxq_qlinear_workspace_size accounts for it); given less,
  * the GEMM runs the DEQUANT kernels. */
-enum { LTXQ_COMPUTE_DEQUANT = 0, LTXQ_COMPUTE_MX2 = 1, LTXQ_COMPUTE_MX1 = 2 };
+/*  FP4 (mxfp4 / nvfp4 weights, standard layout): the activations are quantized
+ *    to the weight's format (ltxq_fp4_quantize, global_scale 1) and the two
+ *    quantized operands multiplied, at every M.  Needs the repacked weight
+ *    scales (mx_scales from ltxq_fp4_pack_weight_scales) and the workspace
+ *    that ltxq_qlinear_workspace_size returns; less is LTXQ_ERR_INVALID.
+ *    4-bit activations do not meet this path's stated tolerance against the
+ *    reference (opt-in). */
+enum { LTXQ_COMPUTE_DEQUANT = 0, LTXQ_COMPUTE_MX2 = 1, LTXQ_COMPUTE_MX1 = 2, LTXQ_COMPUTE_FP4 = 3 };
 
 /* A quantized linear layer in the reference's MLX cache layout
  * (loader/transformer_cache.py:1238-1267, 1436-1462).
  *  affine:  weight uint32 [N, K*bits/32], scales/biases bf16 [N, K/gs]
  *  mxfp8:   weight uint32 [N, K/4] (E4M3), scales uint8 E8M0 [N, K/32]
+ *  mxfp4:   weight uint32 [N, K/8] (E2M1, low nibble first), scales uint8 E8M0
+ *           [N, K/32]: w = code * 2^(scale - 127)
+ *  nvfp4:   weight as mxfp4, scales uint8 E4M3 [N, K/16]:
+ *           w = code * scale * global_scale
+ *  A NaN scale (0xFF E8M0, 0x7F E4M3) makes its whole group NaN; the
+ *  quantizer writes it for a group that holds an infinity or a NaN, which
+ *  E2M1 has no code for.
  *  pretransposed layout: the same arrays built from W^T, i.e. weight
  *  [K, N*bits/32] and scales [K, N/gs] (groups along N).
  *  bias: optional bf16 [N] (the Linear bias, stored unquantized). */
 typedef struct {
   const void* weight;
   const void* scales;
-  const void* biases; /* affine only; NULL for mxfp8 */
+  const void* biases; /* affine only; NULL for the others */
   const void* bias;   /* optional */
   int64_t n_out;
   int64_t k_in;
-  int32_t mode;       /* LTXQ_AFFINE / LTXQ_MXFP8 */
+  int32_t mode;       /* LTXQ_AFFINE / LTXQ_MXFP8 / LTXQ_MXFP4 / LTXQ_NVFP4 */
   int32_t bits;       /* 4 or 8 */
-  int32_t group_size; /* 64 (affine), 32 (mxfp8) */
+  int32_t group_size; /* 64 (affine), 32 (mxfp8, mxfp4), 16 (nvfp4) */
   int32_t layout;     /* LTXQ_LAYOUT_STD / LTXQ_LAYOUT_PRETRANSPOSED */
   uint32_t flags;     /* LTXQ_QW_* (0 = none asserted) */
   int32_t compute;    /* LTXQ_COMPUTE_*: how the GEMM computes (0 = dequantize to bf16) */
   /* LTXQ_COMPUTE_MX*: the weight scales repacked by ltxq_mx_pack_weight_scales
    * (16-byte aligned, ltxq_mx_weight_scales_size bytes); NULL runs the
-   * DEQUANT kernels */
+   * DEQUANT kernels.  LTXQ_COMPUTE_FP4: the scales repacked by
+   * ltxq_fp4_pack_weight_scales. */
   const void* mx_scales;
+  /* nvfp4 only (read in no other mode but checked to be 0 or 1 in mxfp4): the
+   * tensor's scale, within [2^-64, 2^64]; 0 stands for 1 */
+  float global_scale;
+  int32_t pad_;
 } ltxq_qweight;
 
 /* Per-channel vectors (AdaLN scale/shift/gate).  Element (row m, channel c)
@@ -224,6 +244,39 @@ ltxq_status ltxq_qk_norm_rope_pair(const void* q, const void* k, int64_t rows, i
                                    float eps, const float* cos_table, const float* sin_table, int64_t pe_tokens,
                                    void* q_out, void* k_out, void* stream);
 
+/* Rotary positions on one operand of attention (model/transformer/rope.py:53-90
+ * and its interleaved form), the angles formed in the kernel: pair i of head h
+ * of token (b, t) is rotated by position[b, axis[i], t] * freqs[i] (both
+ * indexed [h][i] where freqs_per_head) and multiplied by `scale`.  The pair is
+ * (i, i + rotary_dim/2) in the half layout, (2i, 2i + 1) in the interleaved
+ * one, i < rotary_dim/2; elements past rotary_dim pass through.  `inverse`
+ * rotates back by the same angle with the same scale: the gradient of the
+ * forward call.  Angles are reduced in fp64, the rotation is fp32, one rounding
+ * to the output type.  An axis outside [0, n_axes) gives NaN. */
+enum { LTXQ_ROTARY_HALF = 0, LTXQ_ROTARY_INTERLEAVED = 1 };
+enum { LTXQ_POS_I32 = 0, LTXQ_POS_I64 = 1, LTXQ_POS_F32 = 2, LTXQ_POS_F64 = 3 };
+typedef struct {
+  const void* x;         /* bf16 or f32 [batch, tokens, heads, head_dim], head_dim contiguous */
+  void* out;             /* same type and shape; may be x itself (with x's strides) */
+  int32_t dtype;         /* LTXQ_BF16 / LTXQ_F32 */
+  int32_t layout;        /* LTXQ_ROTARY_* */
+  int64_t batch, tokens, heads, head_dim;
+  int64_t rotary_dim;    /* even, <= head_dim, <= 4096 */
+  int64_t x_stride[3];   /* elements: batch, token, head */
+  int64_t out_stride[3];
+  const void* positions; /* [batch, n_axes, tokens] of pos_dtype */
+  int64_t pos_stride[3]; /* elements: batch, axis, token (0 to share) */
+  int32_t pos_dtype;     /* LTXQ_POS_* */
+  int32_t n_axes;
+  const double* freqs;   /* radians per unit of position: [rotary_dim/2], or [heads][rotary_dim/2] */
+  const int32_t* axis;   /* position axis of each frequency (freqs' shape); NULL: axis 0 */
+  int32_t freqs_per_head;
+  int32_t inverse;
+  float scale;
+  int32_t pad_;
+} ltxq_rotary_args;
+ltxq_status ltxq_rotary(const ltxq_rotary_args* args, void* stream);
+
 /* ---- quantized weights ------------------------------------------------ */
 /* Quantize a bf16 weight [N, K] into the MLX cache layout described by `w`
  * (w->weight/scales/biases are outputs here; w->bias is ignored). */
@@ -315,6 +368,41 @@ ltxq_status ltxq_head_gate_mx(const void* o, const void* logits, int64_t rows, i
  * (attention.py:559-601).  `out_mx` NULL: bf16 `out` only. */
 ltxq_status ltxq_head_gate_ex(const void* o, const void* logits, int64_t logits_stride, int64_t rows, int64_t heads,
                               int64_t head_dim, void* out, const ltxq_mx_act* out_mx, void* stream);
+
+/* A matrix [rows, K] in 4-bit floating point, the input of a product of two
+ * quantized operands: codes [rows, K/2] bytes (low nibble first) and scales in
+ * the block-scaled MMA's atom layout -- with P = 16 (nvfp4) or 8 (mxfp4) groups
+ * per 256 K and row_tiles = ceil(rows / 128), the scale of row t*128 + 32*m1 +
+ * m0, group P*j + 4*a + b at byte (((j * row_tiles + t) * P/4 + a) * 512 +
+ * m0*16 + m1*4 + b); groups past K hold 0, rows past the last are not
+ * written.  Quantization per group: mxfp4 scale 2^e with the largest e >= -127
+ * for which 4 * 2^e <= max|x|; nvfp4 scale RNE_E4M3(max|x| / 6 / global_scale);
+ * codes RNE_E2M1(x / scale), saturating.  Both pointers 16-byte aligned. */
+typedef struct {
+  void* codes;
+  void* scales;
+  int32_t mode;       /* LTXQ_MXFP4 or LTXQ_NVFP4 */
+  float global_scale; /* as in ltxq_qweight */
+} ltxq_fp4_act;
+
+/* row_tiles and the byte sizes of codes and scales; 0 where there is no such
+ * form (K % 32 != 0, an unknown mode, no rows). */
+size_t ltxq_fp4_sizes(int64_t rows, int64_t K, int32_t mode, size_t* codes_bytes, size_t* scale_bytes);
+/* Quantizes bf16 x [M, K] (row stride in elements, a multiple of 8, 16-byte
+ * aligned) into `out`, whose mode and global_scale say how. */
+ltxq_status ltxq_fp4_quantize(const void* x, int64_t M, int64_t K, int64_t row_stride, const ltxq_fp4_act* out,
+                              void* stream);
+/* The values of `a` as bf16 [M, K] (16-byte aligned). */
+ltxq_status ltxq_fp4_dequantize(const ltxq_fp4_act* a, int64_t M, int64_t K, void* out, void* stream);
+/* A weight's row-major scales repacked into the atom layout above, once per
+ * weight; the caller owns the buffer and passes it as ltxq_qweight.mx_scales. */
+size_t ltxq_fp4_weight_scales_size(const ltxq_qweight* w);
+ltxq_status ltxq_fp4_pack_weight_scales(const ltxq_qweight* w, void* out, void* stream);
+/* ltxq_qlinear from quantized activations of the weight's own format:
+ * out = epilogue(dequant(x) . dequant(W)^T).  No workspace.  One quantized x
+ * serves every projection that reads it. */
+ltxq_status ltxq_qlinear_fp4(const ltxq_fp4_act* x, int64_t M, const ltxq_qweight* w, const ltxq_epilogue* epi,
+                             void* out, void* stream);
 
 /* ltxq_adaln_qlinear without a workspace argument and without allocating.
  * No counterpart in the reference.  For hosts that cannot let a library

@@ -28,6 +28,7 @@ struct Params {
   int dp_tiles;
   int splits;
   float* partial;
+  float alpha;  // nvfp4: the tensor scale that multiplies the accumulator (1 elsewhere)
 };
 
 // gelu_approx with the reference's per-op bf16 rounding (feed_forward.py:8-14;
@@ -120,4 +121,8 @@ __device__ __forceinline__ void epi_row_store(const Params& p, uint32_t (&u)[4],
 }
 
 }  // namespace gemm
+
+ltxq_status qlinear_params(const void* x, int64_t M, const ltxq_qweight& w, const ltxq_epilogue* epi, void* out,
+                           gemm::Params* params);
+
 }  // namespace ltxq

@@ -28,6 +28,7 @@
 //     raises the device error word and the CTA unwinds, releasing TMEM.
 #include "common.cuh"
 #include "dequant.cuh"
+#include "fp4.cuh"
 #include "gemm_epilogue.cuh"
 
 namespace ltxq {
@@ -44,6 +45,10 @@ struct Params;
 size_t mx_workspace_bytes(int64_t M, const ltxq_qweight& w);
 ltxq_status launch_qlinear_mx(const void* x, int64_t M, const ltxq_qweight& w, const gemm::Params& p, void* workspace,
                               cudaStream_t stream);
+size_t fp4_workspace_bytes(int64_t M, const ltxq_qweight& w);
+ltxq_status launch_qlinear_fp4_from_bf16(const void* x, int64_t M, const ltxq_qweight& w, const gemm::Params& p,
+                                         void* workspace, cudaStream_t stream);
+ltxq_status fp4_global_scale(int32_t mode, float g, float* out, const char* what);
 
 namespace gemm {
 
@@ -55,12 +60,15 @@ constexpr int kStagePitch = 136;  // epilogue staging row pitch in bf16 (128 + 8
 constexpr int kPrefetch = 2;      // scale/bias register prefetch distance (stages); also the dequant loop's unroll
 
 // kMxfp8F: mxfp8 data flagged LTXQ_QW_MXFP8_FINITE (short conversion)
-enum QKind { kAffine8 = 0, kAffine4 = 1, kMxfp8 = 2, kMxfp8F = 3 };
-constexpr bool is_mx(int qk) { return qk == kMxfp8 || qk == kMxfp8F; }
+enum QKind { kAffine8 = 0, kAffine4 = 1, kMxfp8 = 2, kMxfp8F = 3, kMxfp4 = 4, kNvfp4 = 5 };
+constexpr bool is_fp4(int qk) { return qk == kMxfp4 || qk == kNvfp4; }
+// one byte per group and no biases; groups of 1 << group_log2 elements
+constexpr bool is_mx(int qk) { return qk == kMxfp8 || qk == kMxfp8F || is_fp4(qk); }
+constexpr int group_log2(int qk) { return qk == kNvfp4 ? 4 : 5; }
 
 template <int QK>
 struct QTraits {
-  static constexpr int kWBytes = QK == kAffine4 ? 32 : 64;  // packed bytes per row per stage
+  static constexpr int kWBytes = QK == kAffine4 || is_fp4(QK) ? 32 : 64;  // packed bytes per row per stage
 };
 
 // output tiles of the pair kernel, how many stay whole, K splits of the rest
@@ -81,7 +89,7 @@ struct GroupCursor {
   uint4 cs, cb, ns, nb;
   // g0: the first group get() will be asked for
   __device__ __forceinline__ void init(const Params& p, int64_t srow, bool ok, int g0) {
-    const int gpr = is_mx(QK) ? p.K / 32 : p.K / p.gs;
+    const int gpr = is_mx(QK) ? p.K >> group_log2(QK) : p.K / p.gs;
     nblk = ok ? gpr / kPerBlk : 0;
     sb = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.scales) + srow * (is_mx(QK) ? 1 : 2));
     bb = is_mx(QK) ? nullptr : reinterpret_cast<const uint4*>(p.biases + srow);
@@ -108,7 +116,7 @@ struct GroupCursor {
     if (is_mx(QK)) {
       const int wi = e >> 2;
       const uint32_t w = wi == 0 ? cs.x : wi == 1 ? cs.y : wi == 2 ? cs.z : cs.w;
-      s = (w >> (8 * (e & 3))) & 0xFFu;
+      s = (w >> (8 * (e & 3))) & (QK == kNvfp4 ? 0xFFFFu : 0xFFu);
       b = 0u;
     } else {
       const int wi = e >> 1;
@@ -123,7 +131,8 @@ struct GroupCursor {
 
 // Group parameters of (row n, K-half starting at element k) as the packed
 // form the converters take: affine -> bf16x2 broadcast scale / bias;
-// mxfp8 -> E8M0 byte in `s`.
+// mxfp8 / mxfp4 -> E8M0 byte in `s`; nvfp4 -> the E4M3 bytes of the half's two
+// groups.
 template <int QK>
 __device__ __forceinline__ void load_group(const Params& p, int64_t row_off_scales, int k, bool ok, uint32_t& s,
                                            uint32_t& b) {
@@ -132,7 +141,15 @@ __device__ __forceinline__ void load_group(const Params& p, int64_t row_off_scal
     b = 0u;
     return;
   }
-  if (is_mx(QK)) {
+  if (QK == kNvfp4) {
+    // two groups per K half: bytes, since a row's scales may start anywhere
+    const uint8_t* q = static_cast<const uint8_t*>(p.scales) + row_off_scales + (k >> 4);
+    s = k < p.K ? __ldg(q) | (static_cast<uint32_t>(__ldg(q + 1)) << 8) : 0u;
+    b = 0u;
+  } else if (QK == kMxfp4) {
+    s = k < p.K ? __ldg(static_cast<const uint8_t*>(p.scales) + row_off_scales + (k >> 5)) : 0u;
+    b = 0u;
+  } else if (is_mx(QK)) {
     s = __ldg(static_cast<const uint8_t*>(p.scales) + row_off_scales + (k >> 5));
     b = 0u;
   } else {
@@ -207,14 +224,14 @@ __device__ __forceinline__ void dequant_loop(const Params& p, const Bars& bb, ui
   const int n = n0 + r;
   const bool row_ok = n < p.N;
   const uint32_t t_lane = static_cast<uint32_t>(q * 32) << 16;
-  const int64_t srow = static_cast<int64_t>(n) * (is_mx(QK) ? p.K / 32 : p.K / p.gs);
+  const int64_t srow = static_cast<int64_t>(n) * (is_mx(QK) ? p.K >> group_log2(QK) : p.K / p.gs);
   // group parameters of stage kb live in qs/qb[kb % kPrefetch]; the K loop
   // is unrolled by kPrefetch so every register is read kPrefetch stages
   // after its load was issued (no register moves that would wait on it)
   const bool vec = p.vec_groups != 0;
   const int k_first = kb_first * BK + half * 32;
   GroupCursor<QK> gc;
-  if (vec) gc.init(p, srow, row_ok, is_mx(QK) ? (k_first >> 5) : k_first / p.gs);
+  if (vec) gc.init(p, srow, row_ok, is_mx(QK) ? (k_first >> group_log2(QK)) : k_first / p.gs);
   uint32_t qs[kPrefetch], qb[kPrefetch];
 #pragma unroll
   for (int i = 0; i < kPrefetch; ++i)
@@ -245,7 +262,7 @@ __device__ __forceinline__ void dequant_loop(const Params& p, const Bars& bb, ui
       uint32_t s_cur = qs[i], b_cur = qb[i];
       if (vec) {
         const int k = k_first + kb * BK;
-        gc.get(is_mx(QK) ? (k >> 5) : k / p.gs, s_cur, b_cur);
+        gc.get(is_mx(QK) ? (k >> group_log2(QK)) : k / p.gs, s_cur, b_cur);
         if (!row_ok) {
           s_cur = 0u;
           b_cur = 0u;
@@ -266,6 +283,20 @@ __device__ __forceinline__ void dequant_loop(const Params& p, const Bars& bb, ui
         for (int w4 = 0; w4 < 4; ++w4) {
           uint32_t q4[4];
           deq_affine4_word(wv[w4], s_cur, b_cur, q4);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) o[w4 * 4 + t] = q4[t];
+        }
+      } else if (is_fp4(QK)) {
+        // rows as for kAffine4; one scale per half (mxfp4) or per 16 elements (nvfp4)
+        const uint4 v = *reinterpret_cast<const uint4*>(wrow + ((half ^ ((r >> 2) & 1)) << 4));
+        const uint32_t wv[4] = {v.x, v.y, v.z, v.w};
+        uint32_t s2[2];
+        s2[0] = fp4::scale_bf16x2<QK == kNvfp4 ? fp4::kNv : fp4::kMx>(s_cur & 0xFFu);
+        s2[1] = QK == kNvfp4 ? fp4::scale_bf16x2<fp4::kNv>(s_cur >> 8) : s2[0];
+#pragma unroll
+        for (int w4 = 0; w4 < 4; ++w4) {
+          uint32_t q4[4];
+          fp4::decode_word(wv[w4], s2[w4 >> 1], q4);
 #pragma unroll
           for (int t = 0; t < 4; ++t) o[w4 * 4 + t] = q4[t];
         }
@@ -309,11 +340,19 @@ __device__ __forceinline__ void dequant_loop(const Params& p, const Bars& bb, ui
   if (pend_as >= 0) publish(pend_as);
 }
 
+// An accumulator's value: nvfp4 weights enter as code * scale, their tensor
+// scale multiplies the fp32 sum (one product per output, and code * scale
+// stays exact in bf16).
+template <int QK>
+__device__ __forceinline__ float scaled(const Params& p, uint32_t acc) {
+  return QK == kNvfp4 ? __fmul_rn(__uint_as_float(acc), p.alpha) : __uint_as_float(acc);
+}
+
 // Epilogue (warps 0..7): drain this CTA's 128 x BN accumulator, apply the
 // reference's bias / GELU rounding points, transpose through shared memory
 // (warps of `half` h take 32-token chunks c = h, h+2, ...) and write 16-byte
 // coalesced rows with the gated residual fused in.
-template <int BN>
+template <int QK, int BN>
 __device__ __forceinline__ void epilogue(const Params& p, uint8_t* staging, uint32_t tmem, int warp, int lane, int n0,
                                          int m0) {
   const int q = warp & 3;
@@ -334,7 +373,7 @@ __device__ __forceinline__ void epilogue(const Params& p, uint8_t* staging, uint
     tmem_wait_ld();
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
-      float a = rbf16(__uint_as_float(v[j]));
+      float a = rbf16(scaled<QK>(p, v[j]));
       if (p.bias != nullptr) a = rbf16(__fadd_rn(a, bias_n));
       if (p.epi == LTXQ_EPI_GELU) a = gelu_ref(a);
       stg[j * kStagePitch + r] = f32_to_bf16(a);
@@ -392,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * BM;
   const int m0 = blockIdx.y * BN;
-  const int num_kb = p.K / BK;
+  const int num_kb = (p.K + BK - 1) / BK;  // past the end of K, TMA fills zeros (fp4 weights: K % 32 == 0)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -478,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     dequant_loop<QK, S, AS, P::kACol>(p, bb, ws, tmem, warp, lane, n0, num_kb, 0u, 0, 0);
     if (!*bb.abort_flag && mbar_wait(bb.acc_full, 0, bb.abort_flag, p.err)) {
       tc_fence_after();
-      epilogue<BN>(p, xs, tmem, warp, lane, n0, m0);
+      epilogue<QK, BN>(p, xs, tmem, warp, lane, n0, m0);
     }
   }
 
@@ -702,7 +741,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
-  const int num_kb = p.K / BK;
+  const int num_kb = (p.K + BK - 1) / BK;
   const int n_pt = (p.N + 2 * BM - 1) / (2 * BM);
   const int m_tiles = (p.M + BN - 1) / BN;
   const int tiles = n_pt * m_tiles;
@@ -884,7 +923,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
               const int m = m0 + c * 32 + j;
-              if (m < p.M) dst[(c * 32 + j) * kPairTile] = __uint_as_float(v[j]);
+              if (m < p.M) dst[(c * 32 + j) * kPairTile] = scaled<QK>(p, v[j]);
             }
           }
         }
@@ -907,7 +946,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         for (int h2 = 0; h2 < 2; ++h2) {
           uint32_t h[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) h[j] = pack_bf16x2(__uint_as_float(v[h2][2 * j]), __uint_as_float(v[h2][2 * j + 1]));
+          for (int j = 0; j < 16; ++j) h[j] = pack_bf16x2(scaled<QK>(p, v[h2][2 * j]), scaled<QK>(p, v[h2][2 * j + 1]));
           tmem_st_32x32b_x16(tmem + t_lane + P::kCopyCol + (c + h2) * 16, h);
         }
       }
@@ -1445,7 +1484,7 @@ Sched plan_schedule(int64_t M, int64_t N, int64_t K) {
   const int tiles = static_cast<int>(((N + 2 * BM - 1) / (2 * BM)) * ((M + 255) / 256));
   Sched sc{tiles, tiles, 1};
   const int clusters = num_sms() / 2;
-  const int num_kb = static_cast<int>(K / BK);
+  const int num_kb = static_cast<int>((K + BK - 1) / BK);
   if (clusters <= 0) return sc;
   const int rem = tiles % clusters;
   if (rem == 0 || rem * 2 > clusters) return sc;
@@ -1499,10 +1538,10 @@ ltxq_status check_epilogue(const ltxq_epilogue* epi, int64_t M, int64_t N) {
   }
 }
 
-// workspace (may be NULL): room for the split-K partials; with less than
-// splitk_bytes() the GEMM runs unsplit
-ltxq_status launch_qlinear(const void* x, int64_t M, const ltxq_qweight& w, const ltxq_epilogue* epi, void* out,
-                           cudaStream_t stream, void* workspace, size_t workspace_bytes) {
+// Checks a product's arguments and fills the launch parameters every kernel
+// of this path takes.
+ltxq_status qlinear_params(const void* x, int64_t M, const ltxq_qweight& w, const ltxq_epilogue* epi, void* out,
+                           gemm::Params* params) {
   int64_t R, L;
   if (ltxq_status st = check_qweight(w, true, &R, &L)) return st;
   if (!x || !out) return fail(LTXQ_ERR_INVALID, "qlinear: x/out is NULL");
@@ -1510,19 +1549,25 @@ ltxq_status launch_qlinear(const void* x, int64_t M, const ltxq_qweight& w, cons
   const bool pt = w.layout == LTXQ_LAYOUT_PRETRANSPOSED;
   if (pt && w.mode != LTXQ_MXFP8)
     return fail(LTXQ_ERR_UNSUPPORTED, "qlinear: pretransposed weights are mxfp8 only (the cache's only such mode)");
+  const bool f4 = w.mode == LTXQ_MXFP4 || w.mode == LTXQ_NVFP4;
   const int64_t N = w.n_out, K = w.k_in;
-  if (K % gemm::BK != 0) return fail(LTXQ_ERR_UNSUPPORTED, "qlinear: K must be a multiple of 64");
+  if (f4 && K % 32 != 0) return fail(LTXQ_ERR_UNSUPPORTED, "qlinear: K must be a multiple of 32");
+  if (!f4 && K % gemm::BK != 0) return fail(LTXQ_ERR_UNSUPPORTED, "qlinear: K must be a multiple of 64");
   if (N % 8 != 0) return fail(LTXQ_ERR_UNSUPPORTED, "qlinear: N must be a multiple of 8");
   if (M > 0x7FFFFFFF / 2 || N > 0x7FFFFFFF / 2 || K > 0x7FFFFFFF / 2)
     return fail(LTXQ_ERR_UNSUPPORTED, "qlinear: dimension too large");
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 15u)
     return fail(LTXQ_ERR_UNSUPPORTED, "qlinear: x/out must be 16-byte aligned");
+  if (f4 && (reinterpret_cast<uintptr_t>(w.weight) & 15u))
+    return fail(LTXQ_ERR_UNSUPPORTED, "qlinear: weight must be 16-byte aligned");
   if (w.bias && (reinterpret_cast<uintptr_t>(w.bias) & 15u))
     return fail(LTXQ_ERR_UNSUPPORTED, "qlinear: bias must be 16-byte aligned");
   if (ltxq_status st = check_epilogue(epi, M, N)) return st;
-  if (M == 0) return LTXQ_OK;
-
   gemm::Params p{};
+  p.alpha = 1.f;
+  if (f4) {
+    if (ltxq_status st = fp4_global_scale(w.mode, w.global_scale, &p.alpha, "qlinear")) return st;
+  }
   p.M = static_cast<int>(M);
   p.N = static_cast<int>(N);
   p.K = static_cast<int>(K);
@@ -1539,8 +1584,32 @@ ltxq_status launch_qlinear(const void* x, int64_t M, const ltxq_qweight& w, cons
     p.residual = nullptr;
   }
   p.out = static_cast<uint16_t*>(out);
-  p.err = dev_error_word();
-  if (!p.err) return fail(LTXQ_ERR_CUDA, "qlinear: device error word unavailable");
+  if (M > 0) {
+    p.err = dev_error_word();
+    if (!p.err) return fail(LTXQ_ERR_CUDA, "qlinear: device error word unavailable");
+  }
+  *params = p;
+  return LTXQ_OK;
+}
+
+// workspace (may be NULL): room for the split-K partials; with less than
+// splitk_bytes() the GEMM runs unsplit
+ltxq_status launch_qlinear(const void* x, int64_t M, const ltxq_qweight& w, const ltxq_epilogue* epi, void* out,
+                           cudaStream_t stream, void* workspace, size_t workspace_bytes) {
+  gemm::Params p;
+  if (ltxq_status st = qlinear_params(x, M, w, epi, out, &p)) return st;
+  if (M == 0) return LTXQ_OK;
+  const bool pt = w.layout == LTXQ_LAYOUT_PRETRANSPOSED;
+  const bool f4 = w.mode == LTXQ_MXFP4 || w.mode == LTXQ_NVFP4;
+  const int64_t N = w.n_out, K = w.k_in;
+
+  // products of two fp4 operands (LTXQ_COMPUTE_FP4): the workspace holds the quantized activations
+  if (const size_t bytes = fp4_workspace_bytes(M, w)) {
+    if (!workspace || workspace_bytes < bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u))
+      return fail(LTXQ_ERR_INVALID,
+                  "qlinear: LTXQ_COMPUTE_FP4 needs ltxq_qlinear_workspace_size() bytes of 256-byte aligned workspace");
+    return launch_qlinear_fp4_from_bf16(x, M, w, p, workspace, stream);
+  }
 
   // native block-scaled fp8 path (LTXQ_COMPUTE_MX*), when it applies and the
   // workspace holds the split activations
@@ -1550,7 +1619,9 @@ ltxq_status launch_qlinear(const void* x, int64_t M, const ltxq_qweight& w, cons
   }
 
   const int qk = w.mode == LTXQ_MXFP8 ? ((w.flags & LTXQ_QW_MXFP8_FINITE) ? gemm::kMxfp8F : gemm::kMxfp8)
-                                      : (w.bits == 8 ? gemm::kAffine8 : gemm::kAffine4);
+                 : w.mode == LTXQ_MXFP4 ? gemm::kMxfp4
+                 : w.mode == LTXQ_NVFP4 ? gemm::kNvfp4
+                                        : (w.bits == 8 ? gemm::kAffine8 : gemm::kAffine4);
   gemm::Sched sched = gemm::plan_schedule(M, N, K);
   if (sched.splits > 1 && (!workspace || workspace_bytes < gemm::splitk_bytes(M, N, K) ||
                            (reinterpret_cast<uintptr_t>(workspace) & 15u)))
@@ -1569,17 +1640,18 @@ ltxq_status launch_qlinear(const void* x, int64_t M, const ltxq_qweight& w, cons
       return st;
   } else {
     const int wbytes_row = static_cast<int>(K * w.bits / 8);
-    const uint32_t wbox = qk == gemm::kAffine4 ? 32 : 64;
-    const CUtensorMapSwizzle wsw = qk == gemm::kAffine4 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B;
+    const bool four = qk == gemm::kAffine4 || f4;
+    const uint32_t wbox = four ? 32 : 64;
+    const CUtensorMapSwizzle wsw = four ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B;
     if (ltxq_status st =
             encode_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, w.weight, wbytes_row, N, wbytes_row, wbox, gemm::BM, wsw))
       return st;
   }
   {
-    const int64_t gpr = w.mode == LTXQ_MXFP8 ? K / 32 : K / w.group_size;
-    const int64_t per_blk = w.mode == LTXQ_MXFP8 ? 16 : 8;
+    const int64_t gpr = K / w.group_size;
+    const int64_t per_blk = w.mode == LTXQ_AFFINE ? 8 : 16;
     const bool al = (reinterpret_cast<uintptr_t>(w.scales) & 15u) == 0 &&
-                    (w.mode == LTXQ_MXFP8 || (reinterpret_cast<uintptr_t>(w.biases) & 15u) == 0);
+                    (w.mode != LTXQ_AFFINE || (reinterpret_cast<uintptr_t>(w.biases) & 15u) == 0);
     p.vec_groups = (gpr % per_blk == 0 && al) ? 1 : 0;
   }
   p.dp_tiles = sched.dp;
@@ -1593,6 +1665,8 @@ ltxq_status launch_qlinear(const void* x, int64_t M, const ltxq_qweight& w, cons
     case gemm::kAffine8: return gemm::launch_qk<gemm::kAffine8>(bn, tx, tw, p, stream);
     case gemm::kAffine4: return gemm::launch_qk<gemm::kAffine4>(bn, tx, tw, p, stream);
     case gemm::kMxfp8F: return gemm::launch_qk<gemm::kMxfp8F>(bn, tx, tw, p, stream);
+    case gemm::kMxfp4: return gemm::launch_qk<gemm::kMxfp4>(bn, tx, tw, p, stream);
+    case gemm::kNvfp4: return gemm::launch_qk<gemm::kNvfp4>(bn, tx, tw, p, stream);
     default: return gemm::launch_qk<gemm::kMxfp8>(bn, tx, tw, p, stream);
   }
 }
@@ -1623,6 +1697,7 @@ size_t ltxq_qlinear_workspace_size(int64_t M, const ltxq_qweight* w) {
   if (!w || M <= 0) return 0;
   const size_t mx = ltxq::mx_workspace_bytes(M, *w);
   if (mx) return ltxq::align_up(mx);  // the native path runs unsplit
+  if (const size_t f4 = ltxq::fp4_workspace_bytes(M, *w)) return ltxq::align_up(f4);
   return ltxq::align_up(ltxq::gemm::splitk_bytes(M, w->n_out, w->k_in));
 }
 

@@ -7,13 +7,20 @@
 // clip, scales/biases cast to bf16) and the OCP MX v1.0 MXFP8 quantizer
 // (E8M0 shared exponent floor(log2(amax)) - 8, E4M3 RNE with saturation).
 // ltxq_dequantize produces the bf16 weight the GEMM consumes, bit for bit
-// (the same device functions as the GEMM's dequant warps).
+// (the same device functions as the GEMM's dequant warps).  The mxfp4 / nvfp4
+// forms of both are in fp4.cu.
 #include <mutex>
 
 #include "common.cuh"
 #include "dequant.cuh"
 
 namespace ltxq {
+
+ltxq_status fp4_global_scale(int32_t mode, float g, float* out, const char* what);
+ltxq_status launch_fp4_quantize_rows(const uint16_t* x, int64_t R, int64_t L, int32_t mode, float g, uint8_t* codes,
+                                     uint8_t* scales, cudaStream_t s);
+ltxq_status launch_fp4_dequantize_rows(const uint8_t* codes, const uint8_t* scales, int64_t R, int64_t L, int32_t mode,
+                                       float g, uint16_t* out, cudaStream_t s);
 
 // Quantize along the contiguous dimension of a [R, L] bf16 matrix; one
 // thread per group.
@@ -142,8 +149,12 @@ ltxq_status check_qweight(const ltxq_qweight& w, bool need_data, int64_t* R, int
       return fail(LTXQ_ERR_UNSUPPORTED, "qweight: affine group_size must be 32, 64 or 128");
   } else if (w.mode == LTXQ_MXFP8) {
     if (w.bits != 8 || w.group_size != 32) return fail(LTXQ_ERR_UNSUPPORTED, "qweight: mxfp8 needs bits 8, gs 32");
+  } else if (w.mode == LTXQ_MXFP4) {
+    if (w.bits != 4 || w.group_size != 32) return fail(LTXQ_ERR_UNSUPPORTED, "qweight: mxfp4 needs bits 4, gs 32");
+  } else if (w.mode == LTXQ_NVFP4) {
+    if (w.bits != 4 || w.group_size != 16) return fail(LTXQ_ERR_UNSUPPORTED, "qweight: nvfp4 needs bits 4, gs 16");
   } else {
-    return fail(LTXQ_ERR_UNSUPPORTED, "qweight: mode must be affine or mxfp8");
+    return fail(LTXQ_ERR_UNSUPPORTED, "qweight: mode must be affine, mxfp8, mxfp4 or nvfp4");
   }
   const bool pt = w.layout == LTXQ_LAYOUT_PRETRANSPOSED;
   *R = pt ? w.k_in : w.n_out;
@@ -195,6 +206,15 @@ ltxq_status ltxq_quantize(const void* w_bf16, const ltxq_qweight* w, void* strea
   int64_t R, L;
   if (ltxq_status st = check_qweight(*w, true, &R, &L)) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (w->mode == LTXQ_MXFP4 || w->mode == LTXQ_NVFP4) {
+    float g;
+    if (ltxq_status st = fp4_global_scale(w->mode, w->global_scale, &g, "quantize")) return st;
+    if ((reinterpret_cast<uintptr_t>(w_bf16) | reinterpret_cast<uintptr_t>(w->weight)) & 15u)
+      return fail(LTXQ_ERR_UNSUPPORTED, "quantize: the weight and its codes must be 16-byte aligned");
+    return launch_fp4_quantize_rows(static_cast<const uint16_t*>(w_bf16), R, L, w->mode, g,
+                                    static_cast<uint8_t*>(const_cast<void*>(w->weight)),
+                                    static_cast<uint8_t*>(const_cast<void*>(w->scales)), s);
+  }
   const int threads = 256;
   const unsigned blocks = grid_for(R * (L / w->group_size), threads);
   auto* src = static_cast<const uint16_t*>(w_bf16);
@@ -218,6 +238,14 @@ ltxq_status ltxq_dequantize(const ltxq_qweight* w, void* out_bf16, void* stream)
   if (ltxq_status st = check_qweight(*w, true, &R, &L)) return st;
   if (reinterpret_cast<uintptr_t>(out_bf16) & 15u) return fail(LTXQ_ERR_UNSUPPORTED, "dequantize: out not 16B aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (w->mode == LTXQ_MXFP4 || w->mode == LTXQ_NVFP4) {
+    float g;
+    if (ltxq_status st = fp4_global_scale(w->mode, w->global_scale, &g, "dequantize")) return st;
+    if (reinterpret_cast<uintptr_t>(w->weight) & 15u)
+      return fail(LTXQ_ERR_UNSUPPORTED, "dequantize: the codes must be 16-byte aligned");
+    return launch_fp4_dequantize_rows(static_cast<const uint8_t*>(w->weight), static_cast<const uint8_t*>(w->scales), R,
+                                      L, w->mode, g, static_cast<uint16_t*>(out_bf16), s);
+  }
   const int threads = 256;
   auto* wq = static_cast<const uint32_t*>(w->weight);
   auto* bi = static_cast<const uint16_t*>(w->biases);

@@ -13,6 +13,9 @@ Host-side mirror of the reference's interfaces for the path:
     ``ltxq.denoise`` / ``ltxq.perturbations`` (the AV denoise loop, sigma
     schedules, guiders, STG perturbations of components/ and pipelines/)
   * ``ltxq.cache`` / ``ltxq.cache_build`` (loader/transformer_cache.py)
+  * ``ltxq.FP4Tensor`` and the ``mxfp4`` / ``nvfp4`` modes of
+    ``QuantizedLinear`` (4-bit floating point), ``ltxq.rotary`` (rotary
+    positions without tables; frequencies in ``ltxq.rope``)
 The block linears, modulates, gates and the denoise update run in
 ``libltxq.so`` (hand-written CUDA for sm_100a) through its C ABI
 (include/ltxq.h); there is no CPU fallback.
@@ -20,10 +23,11 @@ The block linears, modulates, gates and the denoise update run in
 
 from . import _lib
 from .feed_forward import FeedForward
-from .kernels import adaln_modulate, adaln_norm_fused, gated_add_fused, head_gate
+from .kernels import FP4Tensor, adaln_modulate, adaln_norm_fused, gated_add_fused, head_gate, rotary
 from .quantized_linear import QuantizedLinear, quant_defaults
 
 __all__ = [
+    "FP4Tensor",
     "FeedForward",
     "QuantizedLinear",
     "adaln_modulate",
@@ -31,6 +35,7 @@ __all__ = [
     "gated_add_fused",
     "head_gate",
     "quant_defaults",
+    "rotary",
 ]
 
 

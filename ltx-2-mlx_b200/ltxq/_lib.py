@@ -17,12 +17,14 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libltxq.so"
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_CUDA, ERR_DEVICE = 0, 1, 2, 3, 4
 BF16, F32 = 0, 1
 NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
-AFFINE, MXFP8 = 0, 1
+AFFINE, MXFP8, MXFP4, NVFP4 = 0, 1, 2, 3
 LAYOUT_STD, LAYOUT_PRETRANSPOSED = 0, 1
 QW_MXFP8_FINITE = 1
-COMPUTE_DEQUANT, COMPUTE_MX2, COMPUTE_MX1 = 0, 1, 2
+COMPUTE_DEQUANT, COMPUTE_MX2, COMPUTE_MX1, COMPUTE_FP4 = 0, 1, 2, 3
 EPI_NONE, EPI_GELU, EPI_GATED_RESIDUAL, EPI_GATE_THEN_ADD = 0, 1, 2, 3
 GATED_ADD, GATE_THEN_ADD = 0, 1
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+POS_I32, POS_I64, POS_F32, POS_F64 = 0, 1, 2, 3
 
 
 class QWeight(ctypes.Structure):
@@ -40,6 +42,8 @@ class QWeight(ctypes.Structure):
         ("flags", ctypes.c_uint32),
         ("compute", c_int32),
         ("mx_scales", c_void_p),
+        ("global_scale", c_float),
+        ("pad_", c_int32),
     ]
 
 
@@ -68,6 +72,36 @@ class MxAct(ctypes.Structure):
         ("sf_hi", c_void_p),
         ("sf_lo", c_void_p),
         ("terms", c_int32),
+        ("pad_", c_int32),
+    ]
+
+
+class Fp4Act(ctypes.Structure):
+    _fields_ = [("codes", c_void_p), ("scales", c_void_p), ("mode", c_int32), ("global_scale", c_float)]
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("out", c_void_p),
+        ("dtype", c_int32),
+        ("layout", c_int32),
+        ("batch", c_int64),
+        ("tokens", c_int64),
+        ("heads", c_int64),
+        ("head_dim", c_int64),
+        ("rotary_dim", c_int64),
+        ("x_stride", c_int64 * 3),
+        ("out_stride", c_int64 * 3),
+        ("positions", c_void_p),
+        ("pos_stride", c_int64 * 3),
+        ("pos_dtype", c_int32),
+        ("n_axes", c_int32),
+        ("freqs", c_void_p),
+        ("axis", c_void_p),
+        ("freqs_per_head", c_int32),
+        ("inverse", c_int32),
+        ("scale", c_float),
         ("pad_", c_int32),
     ]
 
@@ -101,6 +135,13 @@ SIGNATURES = {
                                          c_void_p, c_float, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
     "ltxq_attention": (c_int32, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
                                  c_int64, c_int64, c_float, c_void_p, c_void_p]),
+    "ltxq_rotary": (c_int32, [POINTER(RotaryArgs), c_void_p]),
+    "ltxq_fp4_sizes": (c_size_t, [c_int64, c_int64, c_int32, POINTER(c_size_t), POINTER(c_size_t)]),
+    "ltxq_fp4_quantize": (c_int32, [c_void_p, c_int64, c_int64, c_int64, POINTER(Fp4Act), c_void_p]),
+    "ltxq_fp4_dequantize": (c_int32, [POINTER(Fp4Act), c_int64, c_int64, c_void_p, c_void_p]),
+    "ltxq_fp4_weight_scales_size": (c_size_t, [POINTER(QWeight)]),
+    "ltxq_fp4_pack_weight_scales": (c_int32, [POINTER(QWeight), c_void_p, c_void_p]),
+    "ltxq_qlinear_fp4": (c_int32, [POINTER(Fp4Act), c_int64, POINTER(QWeight), POINTER(Epilogue), c_void_p, c_void_p]),
     "ltxq_quantize": (c_int32, [c_void_p, POINTER(QWeight), c_void_p]),
     "ltxq_dequantize": (c_int32, [POINTER(QWeight), c_void_p, c_void_p]),
     "ltxq_qlinear_workspace_size": (c_size_t, [c_int64, POINTER(QWeight)]),

@@ -136,6 +136,107 @@ def mx_output_ok(C: int) -> bool:
     return C % 128 == 0 and C <= 4096
 
 
+FP4_MODES = {"mxfp4": _lib.MXFP4, "nvfp4": _lib.NVFP4}
+
+
+def _on(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one (its stream and
+    launches are the ones used)."""
+    return torch.cuda.device(t.device)
+
+
+class FP4Tensor:
+    """A matrix in 4-bit floating point, the input form of products of two
+    quantized operands (``ltxq_fp4_act``): E2M1 codes [M, K / 2] bytes and
+    group scales in the block-scaled MMA's atom layout.
+
+    ``mode`` "mxfp4": 32 values along K share an E8M0 scale; "nvfp4": 16 share
+    an E4M3 scale, times ``global_scale`` (one number for the tensor).  A group
+    that holds an infinity or a NaN reads back as NaN.  K must be a multiple of
+    32.  Written by ``quantize``, read by ``dequantize`` and by a
+    ``QuantizedLinear`` of the same mode whose compute is "fp4"; one quantized
+    tensor serves every projection that reads it."""
+
+    def __init__(self, rows_shape: tuple[int, ...], K: int, mode: str, device, global_scale: float = 1.0):
+        if mode not in FP4_MODES:
+            raise ValueError(f"mode must be one of {sorted(FP4_MODES)}, got {mode!r}")
+        self.rows_shape = tuple(rows_shape)
+        self.K = int(K)
+        self.mode = mode
+        self.global_scale = float(global_scale)
+        self.M = math.prod(self.rows_shape)
+        if self.K <= 0 or self.K % 32 != 0:
+            raise ValueError(f"K must be a positive multiple of 32, got {self.K}")
+        group = 16 if mode == "nvfp4" else 32
+        if mode != "nvfp4" and self.global_scale != 1.0:
+            raise ValueError("global_scale is nvfp4 only")
+        if not 2.0 ** -64 <= self.global_scale <= 2.0 ** 64:
+            raise ValueError("global_scale must be within [2^-64, 2^64]")
+        self._code_bytes = self.M * (self.K // 2)
+        self._scale_bytes = -(-self.K // 256) * -(-self.M // 128) * 128 * (256 // group)
+        self._scale_off = _align(self._code_bytes)
+        self.buffer = torch.empty(self._scale_off + self._scale_bytes, dtype=torch.uint8, device=device)
+
+    @property
+    def shape(self) -> tuple[int, ...]:
+        return self.rows_shape + (self.K,)
+
+    @property
+    def device(self):
+        return self.buffer.device
+
+    def tensors(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """(codes [M, K / 2], scale atoms flat) as uint8 views of the buffer."""
+        return (self.buffer[:self._code_bytes].view(self.M, self.K // 2),
+                self.buffer[self._scale_off:self._scale_off + self._scale_bytes])
+
+    def struct(self) -> _lib.Fp4Act:
+        base = self.buffer.data_ptr()
+        return _lib.Fp4Act(base, base + self._scale_off, FP4_MODES[self.mode], self.global_scale)
+
+    @classmethod
+    def quantize(cls, x: torch.Tensor, mode: str = "nvfp4", global_scale: float = 1.0) -> "FP4Tensor":
+        """bf16 ``x`` (..., K) quantized along K."""
+        _require_cuda(x, "x")
+        if x.dtype != torch.bfloat16:
+            raise ValueError(f"x must be bfloat16, got {x.dtype}")
+        if x.dim() < 1:
+            raise ValueError("x must have at least one dimension")
+        with _on(x):
+            t = cls(tuple(x.shape[:-1]), x.shape[-1], mode, x.device, global_scale)
+            if t.M == 0:
+                return t
+            if x.dim() != 2 or x.stride(1) != 1 or x.stride(0) % 8 != 0 or x.stride(0) < t.K or x.data_ptr() % 16:
+                x = x.reshape(t.M, t.K)  # rows at one stride; copied where they are not
+                if x.stride(1) != 1 or x.stride(0) % 8 != 0 or x.stride(0) < t.K or x.data_ptr() % 16:
+                    x = x.clone(memory_format=torch.contiguous_format)
+            st = t.struct()
+            _lib.check(_lib.load().ltxq_fp4_quantize(x.data_ptr(), t.M, t.K, x.stride(0) if t.M > 1 else t.K,
+                                                     ctypes.byref(st), _stream()), "fp4_quantize")
+        return t
+
+    def dequantize(self) -> torch.Tensor:
+        """The values, as bf16 of the quantized tensor's shape."""
+        with _on(self.buffer):
+            out = torch.empty(self.shape, dtype=torch.bfloat16, device=self.device)
+            if self.M:
+                st = self.struct()
+                _lib.check(_lib.load().ltxq_fp4_dequantize(ctypes.byref(st), self.M, self.K, out.data_ptr(), _stream()),
+                           "fp4_dequantize")
+        return out
+
+
+def fp4_global_scale(x: torch.Tensor) -> float:
+    """A ``global_scale`` for quantizing ``x`` to nvfp4: the power of two that
+    puts the scale of the group with the largest magnitude just inside E4M3's
+    range (448), so that small weights do not fall into its subnormals.  Reads
+    one number back from the device."""
+    amax = float(x.detach().abs().amax()) if x.numel() else 0.0
+    if not math.isfinite(amax) or amax == 0.0:
+        return 1.0
+    return 2.0 ** max(-64, min(64, math.ceil(math.log2(amax / (6.0 * 448.0)))))
+
+
 def prologue(norm: int, eps: float, scale, shift, rows_shape, C, keep) -> _lib.Prologue:
     return _lib.Prologue(norm, float(eps), vec_arg(scale, rows_shape, C, "scale", keep),
                          vec_arg(shift, rows_shape, C, "shift", keep))
@@ -326,4 +427,91 @@ def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, heads: int, eps: float =
                                              cos.data_ptr() if cos is not None else None,
                                              sin.data_ptr() if sin is not None else None, t, out.data_ptr(),
                                              _stream()), "qk_norm_rope")
+    return out
+
+
+_POS = {torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64, torch.float32: _lib.POS_F32, torch.float64: _lib.POS_F64}
+_ROTARY_LAYOUT = {"half": _lib.ROTARY_HALF, "interleaved": _lib.ROTARY_INTERLEAVED}
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, heads: int, *, layout: str = "half",
+           axes: torch.Tensor | None = None, scale: float = 1.0, inverse: bool = False,
+           out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions on one operand of attention, the angles formed in the
+    kernel (no cos / sin tables): pair i of a head turns by ``positions *
+    freqs[i]`` and is multiplied by ``scale``.
+
+    ``x``: bf16 or fp32, (B, T, heads*D) or (B, T, heads, D), any strides with
+    a unit last one (a column slice of a fused projection, a transposed
+    (B, heads, T, D)).  ``layout`` "half" pairs elements i and i + R/2 of a
+    head (the split form of rope.py:53-90), "interleaved" 2i and 2i + 1, with
+    R = 2 * freqs.shape[-1] <= D; elements past R pass through.  ``freqs``:
+    float64, radians per unit of position, (R/2,) or (heads, R/2)
+    (``rope.rotary_frequencies``, ``rope.grid_rotary``).  ``positions``:
+    int32, int64, float32 or float64, (T,) or (B, T); with ``axes`` (int32,
+    freqs' shape: the position axis of each frequency) (A, T) or (B, A, T).
+    An axis outside [0, A) gives NaN.
+
+    ``inverse`` turns back by the same angles with the same scale: the
+    gradient of the forward call.  ``out`` (x's shape and type) may be ``x``.
+    Returns ``out``, contiguous where it is made here."""
+    _require_cuda(x, "x")
+    _require_cuda(positions, "positions")
+    _require_cuda(freqs, "freqs")
+    if x.dtype not in _DT:
+        raise ValueError(f"x dtype must be bfloat16 or float32, got {x.dtype}")
+    if layout not in _ROTARY_LAYOUT:
+        raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+    if heads <= 0 or x.dim() not in (3, 4) or (x.dim() == 4 and x.shape[2] != heads):
+        raise ValueError(f"x must be (B, T, {heads} * D) or (B, T, {heads}, D), got {tuple(x.shape)}")
+    if x.dim() == 3 and x.shape[2] % heads != 0:
+        raise ValueError("x's last dimension must be a multiple of heads")
+    b, t = x.shape[0], x.shape[1]
+    d = x.shape[3] if x.dim() == 4 else x.shape[2] // heads
+    if freqs.dtype != torch.float64 or freqs.dim() not in (1, 2) or (freqs.dim() == 2 and freqs.shape[0] != heads):
+        raise ValueError(f"freqs must be float64 (R/2,) or ({heads}, R/2), got {freqs.dtype} {tuple(freqs.shape)}")
+    r = 2 * freqs.shape[-1]
+    if r > d:
+        raise ValueError(f"freqs rotate {r} elements but a head has {d}")
+    if positions.dtype not in _POS:
+        raise ValueError(f"positions must be int32, int64, float32 or float64, got {positions.dtype}")
+    lead = positions.dim() - (1 if axes is None else 2)
+    if lead not in (0, 1) or positions.shape[-1] != t or (lead and positions.shape[0] != b):
+        raise ValueError(f"positions shape {tuple(positions.shape)} does not match {b} x {t} tokens")
+    n_axes = 1
+    if axes is not None:
+        _require_cuda(axes, "axes")
+        if axes.dtype != torch.int32 or axes.shape != freqs.shape:
+            raise ValueError("axes must be int32 with the shape of freqs")
+        n_axes = positions.shape[-2]
+        axes = axes.contiguous()
+        if n_axes < 1:
+            raise ValueError("positions have no axis")
+    for o, name in ((positions, "positions"), (freqs, "freqs"), (axes, "axes"), (out, "out")):
+        if o is not None and o.device != x.device:
+            raise ValueError(f"{name} is on {o.device}, x on {x.device}")
+    if d == 0:
+        raise ValueError("heads have no elements")
+    with _on(x):
+        if x.stride(-1) != 1 and x.shape[-1] > 1:
+            if out is x:
+                raise ValueError("an in-place rotation needs x with a unit last stride")
+            x = x.contiguous()
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        elif out.shape != x.shape or out.dtype != x.dtype or (out.stride(-1) != 1 and out.shape[-1] > 1):
+            raise ValueError("out must have x's shape and type and a unit last stride")
+        if x.numel() == 0:
+            return out
+        freqs = freqs.contiguous()
+        st = _lib.RotaryArgs(x=x.data_ptr(), out=out.data_ptr(), dtype=_DT[x.dtype], layout=_ROTARY_LAYOUT[layout],
+                             batch=b, tokens=t, heads=heads, head_dim=d, rotary_dim=r,
+                             positions=positions.data_ptr(), pos_dtype=_POS[positions.dtype], n_axes=n_axes,
+                             freqs=freqs.data_ptr(), axis=axes.data_ptr() if axes is not None else None,
+                             freqs_per_head=int(freqs.dim() == 2), inverse=int(bool(inverse)), scale=float(scale))
+        st.x_stride[:] = (x.stride(0), x.stride(1), x.stride(2) if x.dim() == 4 else d)
+        st.out_stride[:] = (out.stride(0), out.stride(1), out.stride(2) if out.dim() == 4 else d)
+        st.pos_stride[:] = (positions.stride(0) if lead else 0, positions.stride(-2) if axes is not None else 0,
+                            positions.stride(-1))
+        _lib.check(_lib.load().ltxq_rotary(ctypes.byref(st), _stream()), "rotary")
     return out

@@ -7,7 +7,9 @@ it (LTX_2_MLX/loader/transformer_cache.py:1436-1462 builds the empty module,
 ``mode``/``group_size``/``bits`` semantics and defaults (:797-811), and
 ``__call__(x) -> y``.  ``pretransposed=True`` gives the reference's
 ``_PretransposedQuantizedLinear`` (:177-193) whose packed arrays were built
-from ``W.T``.
+from ``W.T``.  The 4-bit floating point modes "mxfp4" and "nvfp4" (the
+reference's defaults 32/4 and 16/4) compute either from the dequantized weight
+or, with ``set_compute("fp4")``, as a product of two quantized operands.
 
 The forward pass is one launch of the sm_100a quantized GEMM with the
 block's epilogue fused (bias, GELU, gated residual); there is no CPU path.
@@ -21,14 +23,17 @@ import math
 import torch
 
 from . import _lib
-from .kernels import MXActivation, _require_cuda, _stream, prologue, vec_arg
+from .kernels import FP4_MODES, FP4Tensor, MXActivation, _on, _require_cuda, _stream, prologue, vec_arg
 
-QUANT_DEFAULTS = {"affine": (64, 4), "mxfp8": (32, 8)}
-_MODE = {"affine": _lib.AFFINE, "mxfp8": _lib.MXFP8}
+QUANT_DEFAULTS = {"affine": (64, 4), "mxfp8": (32, 8), "mxfp4": (32, 4), "nvfp4": (16, 4)}
+_MODE = {"affine": _lib.AFFINE, "mxfp8": _lib.MXFP8, **FP4_MODES}
 # how the GEMM computes (include/ltxq.h LTXQ_COMPUTE_*): "dequant" (bf16
 # tensor cores over the exactly dequantized weight), "mx2" / "mx1" (native
-# block-scaled fp8 MMAs on mxfp8 weights, activations in two / one MXFP8 terms)
-COMPUTE = {"dequant": _lib.COMPUTE_DEQUANT, "mx2": _lib.COMPUTE_MX2, "mx1": _lib.COMPUTE_MX1}
+# block-scaled fp8 MMAs on mxfp8 weights, activations in two / one MXFP8 terms),
+# "fp4" (block-scaled fp4 MMAs on mxfp4 / nvfp4 weights, activations quantized
+# to the weight's format)
+COMPUTE = {"dequant": _lib.COMPUTE_DEQUANT, "mx2": _lib.COMPUTE_MX2, "mx1": _lib.COMPUTE_MX1,
+           "fp4": _lib.COMPUTE_FP4}
 
 
 def quant_defaults(mode: str, group_size: int | None, bits: int | None) -> tuple[int, int]:
@@ -43,9 +48,15 @@ def quant_defaults(mode: str, group_size: int | None, bits: int | None) -> tuple
 class QuantizedLinear:
     def __init__(self, weight: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor | None = None,
                  bias: torch.Tensor | None = None, *, group_size: int, bits: int, mode: str = "affine",
-                 pretransposed: bool = False, in_features: int | None = None, out_features: int | None = None):
+                 pretransposed: bool = False, in_features: int | None = None, out_features: int | None = None,
+                 global_scale: float = 1.0):
         if mode not in _MODE:
             raise ValueError(f"Unsupported quantization mode: {mode}")
+        if mode != "nvfp4" and global_scale != 1.0:
+            raise ValueError("global_scale is nvfp4 only")
+        if not 2.0 ** -64 <= global_scale <= 2.0 ** 64:
+            raise ValueError("global_scale must be within [2^-64, 2^64]")
+        self.global_scale = float(global_scale)
         for t, name in ((weight, "weight"), (scales, "scales")):
             _require_cuda(t, name)
         self.weight = weight.contiguous()
@@ -70,8 +81,8 @@ class QuantizedLinear:
 
     def set_compute(self, compute: str) -> "QuantizedLinear":
         """Select how GEMMs over this weight compute (``COMPUTE``); the MX
-        modes apply to mxfp8 weights in the standard layout, other weights
-        keep the dequantizing kernels."""
+        modes apply to mxfp8 weights and "fp4" to mxfp4 / nvfp4 weights, both
+        in the standard layout; other weights keep the dequantizing kernels."""
         if compute not in COMPUTE:
             raise ValueError(f"unknown compute mode {compute!r}")
         self.compute = compute
@@ -81,10 +92,25 @@ class QuantizedLinear:
         return self
 
     def mx_scales(self) -> torch.Tensor | None:
-        """The weight scales repacked for the MX modes' block-scaled MMA
-        (``ltxq_mx_pack_weight_scales``), made once and again only when the
-        scale tensor changes; None where the MX modes do not apply."""
-        if getattr(self, "compute", "dequant") == "dequant" or self.mode != "mxfp8" or self.pretransposed:
+        """The weight scales repacked for the block-scaled MMA of the MX modes
+        (``ltxq_mx_pack_weight_scales``) or of "fp4"
+        (``ltxq_fp4_pack_weight_scales``), made once and again only when the
+        scale tensor changes; None where those modes do not apply."""
+        if self.computes_fp4():
+            key = (self.scales.data_ptr(), self.scales._version)
+            cached = getattr(self, "_mx_scales", None)
+            if cached is None or cached[0] != key:
+                with _on(self.scales):
+                    lib = _lib.load()
+                    q = self._qweight_base(0, None)
+                    buf = torch.empty(lib.ltxq_fp4_weight_scales_size(ctypes.byref(q)), dtype=torch.uint8,
+                                      device=self.scales.device)
+                    _lib.check(lib.ltxq_fp4_pack_weight_scales(ctypes.byref(q), buf.data_ptr(), _stream()),
+                               "fp4_pack_weight_scales")
+                cached = (key, buf)
+                self._mx_scales = cached
+            return cached[1]
+        if getattr(self, "compute", "dequant") in ("dequant", "fp4") or self.mode != "mxfp8" or self.pretransposed:
             return None
         if self.in_features % 512 != 0:
             return None
@@ -100,13 +126,31 @@ class QuantizedLinear:
             self._mx_scales = cached
         return cached[1]
 
+    def computes_fp4(self) -> bool:
+        """Whether products over this weight are of two fp4 operands."""
+        return (getattr(self, "compute", "dequant") == "fp4" and self.mode in FP4_MODES and not self.pretransposed
+                and self.in_features % 32 == 0)
+
     # ------------------------------------------------------------------ build
     @classmethod
     def from_linear(cls, weight: torch.Tensor, bias: torch.Tensor | None = None, group_size: int | None = None,
-                    bits: int | None = None, mode: str = "affine", pretransposed: bool = False) -> "QuantizedLinear":
+                    bits: int | None = None, mode: str = "affine", pretransposed: bool = False,
+                    global_scale: float = 1.0) -> "QuantizedLinear":
         """Quantize a bf16 ``nn.Linear`` weight [out, in] on the GPU
-        (``nn.QuantizedLinear.from_linear`` / ``mx.quantize``)."""
+        (``nn.QuantizedLinear.from_linear`` / ``mx.quantize``).
+        ``global_scale`` (nvfp4): the tensor's scale, as
+        ``kernels.fp4_global_scale(weight)`` picks one; 1 is the reference's
+        cache layout, which has none."""
         _require_cuda(weight, "weight")
+        if mode in FP4_MODES:
+            with _on(weight):
+                return cls._from_linear(weight, bias, group_size, bits, mode, pretransposed, global_scale)
+        if global_scale != 1.0:
+            raise ValueError("global_scale is nvfp4 only")
+        return cls._from_linear(weight, bias, group_size, bits, mode, pretransposed, 1.0)
+
+    @classmethod
+    def _from_linear(cls, weight, bias, group_size, bits, mode, pretransposed, global_scale):
         gs, b = quant_defaults(mode, group_size, bits)
         w = weight.to(torch.bfloat16)
         n_out, k_in = w.shape
@@ -121,11 +165,11 @@ class QuantizedLinear:
             biases = None
         q = _lib.QWeight(packed.data_ptr(), scales.data_ptr(), biases.data_ptr() if biases is not None else None,
                          None, n_out, k_in, _MODE[mode], b, gs,
-                         _lib.LAYOUT_PRETRANSPOSED if pretransposed else _lib.LAYOUT_STD)
+                         _lib.LAYOUT_PRETRANSPOSED if pretransposed else _lib.LAYOUT_STD, global_scale=global_scale)
         _lib.check(_lib.load().ltxq_quantize(src.data_ptr(), ctypes.byref(q), _stream()), "quantize")
         bias_bf16 = bias.to(torch.bfloat16).contiguous() if bias is not None else None
         return cls(packed, scales, biases, bias_bf16, group_size=gs, bits=b, mode=mode,
-                   pretransposed=pretransposed, in_features=k_in, out_features=n_out)
+                   pretransposed=pretransposed, in_features=k_in, out_features=n_out, global_scale=global_scale)
 
     # ------------------------------------------------------------------ views
     def _qweight_base(self, flags: int, mx_scales) -> _lib.QWeight:
@@ -135,7 +179,7 @@ class QuantizedLinear:
             self.bias.data_ptr() if self.bias is not None else None,
             self.out_features, self.in_features, _MODE[self.mode], self.bits, self.group_size,
             _lib.LAYOUT_PRETRANSPOSED if self.pretransposed else _lib.LAYOUT_STD, flags,
-            COMPUTE[getattr(self, "compute", "dequant")], mx_scales)
+            COMPUTE[getattr(self, "compute", "dequant")], mx_scales, getattr(self, "global_scale", 1.0))
 
     def qweight(self) -> _lib.QWeight:
         mx = self.mx_scales()
@@ -165,13 +209,18 @@ class QuantizedLinear:
         shape = (self.in_features, self.out_features) if self.pretransposed else (self.out_features, self.in_features)
         out = torch.empty(shape, dtype=torch.bfloat16, device=self.weight.device)
         q = self.qweight()
+        if self.mode in FP4_MODES:
+            with _on(self.weight):
+                _lib.check(_lib.load().ltxq_dequantize(ctypes.byref(q), out.data_ptr(), _stream()), "dequantize")
+            return out
         _lib.check(_lib.load().ltxq_dequantize(ctypes.byref(q), out.data_ptr(), _stream()), "dequantize")
         return out
 
     def mx_terms(self, M: int) -> int:
         """Terms of the MX input a GEMM of M rows over this weight takes (2 for
-        "mx2", 1 for "mx1"), or 0 where it runs the dequantizing kernels."""
-        if self.compute == "dequant" or M <= 0:
+        "mx2", 1 for "mx1"), or 0 where it runs the dequantizing kernels (or
+        the fp4 ones)."""
+        if self.compute in ("dequant", "fp4") or M <= 0:
             return 0
         q = self.qweight()
         if not _lib.load().ltxq_qlinear_mx_supported(M, ctypes.byref(q)):
@@ -211,7 +260,23 @@ class QuantizedLinear:
         ``x`` may be an ``MXActivation`` (``mx_terms(M)`` terms): the
         block-scaled GEMM reads it directly (``ltxq_qlinear_mx``).  With such
         an input, ``mx_out`` 1 or 2 returns the result (bias, GELU applied) as
-        an ``MXActivation`` of that many terms for the next GEMM."""
+        an ``MXActivation`` of that many terms for the next GEMM.
+
+        With compute "fp4" on an mxfp4 / nvfp4 weight, ``x`` is quantized to
+        the weight's format in the call, or comes as an ``FP4Tensor`` of it."""
+        if isinstance(x, FP4Tensor) or self.mode in FP4_MODES:
+            if mx_out:
+                raise ValueError("mx_out needs an MXActivation input (the block-scaled fp8 kernels)")
+            dev = x.device
+            if dev != self.weight.device:
+                raise ValueError(f"x is on {dev}, the weight on {self.weight.device}")
+            if isinstance(x, FP4Tensor):
+                with _on(self.weight):
+                    return self._call_fp4(x, gelu, residual, gate, gate_then_add, adaln)
+            if dev.index != torch.cuda.current_device() and dev.type == "cuda":
+                with _on(self.weight):
+                    return self(x, gelu=gelu, residual=residual, gate=gate, gate_then_add=gate_then_add, adaln=adaln,
+                                split_k=split_k)
         if isinstance(x, MXActivation):
             return self._call_mx(x, gelu, residual, gate, gate_then_add, mx_out)
         if mx_out:
@@ -227,6 +292,8 @@ class QuantizedLinear:
         keep: list = []
         epi = self._epilogue(rows_shape, keep, gelu, residual, gate, gate_then_add)
         out = torch.empty(rows_shape + (self.out_features,), dtype=torch.bfloat16, device=x.device)
+        if M == 0:
+            return out
         q = self.qweight()
         lib = _lib.load()
         if adaln is not None:
@@ -239,10 +306,28 @@ class QuantizedLinear:
             _lib.check(lib.ltxq_adaln_qlinear(x.data_ptr(), M, ctypes.byref(pro), ctypes.byref(q), ctypes.byref(epi),
                                               out.data_ptr(), ws.data_ptr(), ws_bytes, _stream()), "adaln_qlinear")
         else:
-            ws_bytes = lib.ltxq_qlinear_workspace_size(M, ctypes.byref(q)) if split_k else 0
+            ws_bytes = (lib.ltxq_qlinear_workspace_size(M, ctypes.byref(q)) if split_k or self.computes_fp4() else 0)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
             _lib.check(lib.ltxq_qlinear(x.data_ptr(), M, ctypes.byref(q), ctypes.byref(epi), out.data_ptr(),
                                         ws.data_ptr() if ws is not None else None, ws_bytes, _stream()), "qlinear")
+        return out
+
+    def _call_fp4(self, x: FP4Tensor, gelu, residual, gate, gate_then_add, adaln):
+        if not self.computes_fp4() or x.mode != self.mode:
+            raise ValueError(f"an {x.mode} input needs an {x.mode} weight whose compute is 'fp4' (weight: {self.mode}, "
+                             f"compute: {self.compute})")
+        if adaln is not None:
+            raise ValueError("adaln takes bf16 activations")
+        if x.K != self.in_features:
+            raise ValueError(f"x last dim {x.K} != in_features {self.in_features}")
+        keep: list = []
+        epi = self._epilogue(x.rows_shape, keep, gelu, residual, gate, gate_then_add)
+        out = torch.empty(x.rows_shape + (self.out_features,), dtype=torch.bfloat16, device=x.device)
+        if x.M == 0:
+            return out
+        q, xs = self.qweight(), x.struct()
+        _lib.check(_lib.load().ltxq_qlinear_fp4(ctypes.byref(xs), x.M, ctypes.byref(q), ctypes.byref(epi),
+                                                out.data_ptr(), _stream()), "qlinear_fp4")
         return out
 
     def _call_mx(self, x: MXActivation, gelu, residual, gate, gate_then_add, mx_out):

@@ -10,7 +10,8 @@ token, in pixels for height / width and in seconds for time.
 
 Everything here is table arithmetic in torch (fp32, or a float64 frequency
 grid), computed once per stage on the tensors' device; the per-step rotation
-itself is ``ltxq_qk_norm_rope``.
+itself is ``ltxq_qk_norm_rope``, or ``ltxq_rotary``, which forms the angles in
+the kernel from what ``rotary_frequencies`` and ``grid_rotary`` make.
 """
 
 from __future__ import annotations
@@ -103,3 +104,78 @@ def audio_positions(batch: int, frames: int, sample_rate: int = 16000, hop_lengt
 
     pos = torch.stack([times(shift, frames + shift), times(shift + 1, frames + shift + 1)], dim=-1)
     return pos[None, None].expand(batch, 1, -1, -1).contiguous()
+
+
+def rotary_frequencies(rotary_dim: int, theta: float = THETA, *, scaling: str = "none", factor: float = 1.0,
+                       original_length: int | None = None, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                       device=None) -> tuple[torch.Tensor, float]:
+    """(freqs, scale) for ``kernels.rotary``: float64 (rotary_dim / 2,)
+    frequencies theta^(-2i / rotary_dim) and the factor on the rotated vector.
+
+    ``scaling`` stretches them for contexts ``factor`` times longer:
+    "linear" divides every position by ``factor`` (position interpolation,
+    Chen et al. 2023); "ntk" raises theta to theta * factor^(R / (R - 2)), which
+    keeps the fastest frequency and divides the slowest by ``factor``; "yarn"
+    (Peng et al. 2023) keeps the frequencies that make more than ``beta_fast``
+    turns over ``original_length`` positions, divides those below
+    ``beta_slow`` turns by ``factor``, blends linearly in the number of turns
+    between, and scales the vector by 0.1 ln(factor) + 1."""
+    if rotary_dim <= 0 or rotary_dim % 2 != 0:
+        raise ValueError(f"rotary_dim must be positive and even, got {rotary_dim}")
+    if scaling not in ("none", "linear", "ntk", "yarn"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    if not (theta > 0 and factor >= 1.0 and math.isfinite(theta) and math.isfinite(factor)):
+        raise ValueError("theta must be positive and factor at least 1")
+    if scaling == "none" and factor != 1.0:
+        raise ValueError("factor needs a scaling")
+    base = theta
+    if scaling == "ntk":
+        if rotary_dim == 2:
+            raise ValueError("ntk scaling needs rotary_dim > 2")
+        base = theta * factor ** (rotary_dim / (rotary_dim - 2))
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    f = base ** (-2.0 * i / rotary_dim)
+    scale = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        if original_length is None or original_length <= 0 or not beta_fast > beta_slow:
+            raise ValueError("yarn scaling needs original_length and beta_fast > beta_slow")
+        turns = original_length * f / (2 * math.pi)
+        keep = ((turns - beta_slow) / (beta_fast - beta_slow)).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1 - keep)
+        scale = 0.1 * math.log(factor) + 1.0
+    return f.to(device), scale
+
+
+def grid_rotary(indices_grid: torch.Tensor, dim: int, theta: float = THETA, max_pos=VIDEO_MAX_POS,
+                use_middle_indices_grid: bool = False, num_attention_heads: int = 32
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(positions, freqs, axes) with which ``kernels.rotary(x, positions,
+    freqs, heads, axes=axes)`` turns as the tables of ``precompute_freqs_cis``
+    (the same arguments) do, without the tables: positions float64 (B, n_dims,
+    T), scaled to [-1, 1] per dimension; freqs float64 and axes int32 (heads,
+    dim / 2 / heads).  The padded front has frequency 0 (the identity)."""
+    g = indices_grid.double()
+    n_dims = g.shape[1]
+    if len(max_pos) != n_dims:
+        raise ValueError(f"{n_dims} position dimensions but max_pos has {len(max_pos)}")
+    if use_middle_indices_grid:
+        if g.dim() != 4 or g.shape[-1] != 2:
+            raise ValueError("use_middle_indices_grid needs (B, n_dims, T, 2) bounds")
+        g = (g[..., 0] + g[..., 1]) / 2.0
+    elif g.dim() == 4:
+        g = g[..., 0]
+    if dim % (2 * num_attention_heads) != 0:
+        raise ValueError("dim must be a multiple of 2 * num_attention_heads")
+    limits = torch.tensor(max_pos, dtype=torch.float64, device=g.device).view(1, n_dims, 1)
+    n = dim // (2 * n_dims)
+    t = torch.arange(n, dtype=torch.float64, device=g.device) / max(n - 1, 1)
+    f = torch.pow(torch.tensor(theta, dtype=torch.float64, device=g.device), t) * (math.pi / 2)
+    freqs = torch.zeros(dim // 2, dtype=torch.float64, device=g.device)
+    axes = torch.zeros(dim // 2, dtype=torch.int32, device=g.device)
+    pad = dim // 2 - n * n_dims
+    freqs[pad:] = f.repeat_interleave(n_dims)
+    axes[pad:] = torch.arange(n_dims, dtype=torch.int32, device=g.device).repeat(n)
+    shape = (num_attention_heads, dim // 2 // num_attention_heads)
+    return (2 * g / limits - 1).contiguous(), freqs.view(shape), axes.view(shape)
