@@ -16,6 +16,9 @@ namespace ltxq {
 
 ltxq_status check_qweight(const ltxq_qweight& w, bool need_data, int64_t* R, int64_t* L);
 ltxq_status check_epilogue(const ltxq_epilogue* epi, int64_t M, int64_t N);
+bool fp4_rows_supported(int64_t M, const ltxq_qweight& w);
+ltxq_status launch_fp4_rows(const void* x, bool quantize, const ltxq_fp4_act* packed, const ltxq_qweight& w,
+                            const gemm::Params& p, cudaStream_t stream);
 
 namespace fp4 {
 
@@ -577,6 +580,7 @@ static ltxq_status launch_gemm(const ltxq_fp4_act& x, const ltxq_qweight& w, con
 // (codes, then scale atoms), or 0 where `w` does not compute in fp4.
 size_t fp4_workspace_bytes(int64_t M, const ltxq_qweight& w) {
   if (w.compute != LTXQ_COMPUTE_FP4 || !fp4::is_fp4(w.mode) || w.layout != LTXQ_LAYOUT_STD) return 0;
+  if (fp4_rows_supported(M, w)) return 0;  // the few-row kernel quantizes as it reads
   if (M <= 0 || w.k_in <= 0 || w.k_in % 32 != 0) return 0;
   const fp4::Sizes s = fp4::sizes(M, w.k_in, w.mode);
   return fp4::align_up(s.codes) + fp4::align_up(s.scales);
@@ -588,6 +592,11 @@ ltxq_status launch_qlinear_fp4(const ltxq_fp4_act& x, int64_t M, const ltxq_qwei
   if (ltxq_status st = fp4::check_act(&x, M, w.k_in, &gx, "qlinear_fp4")) return st;
   if (ltxq_status st = fp4_global_scale(w.mode, w.global_scale, &gw, "qlinear_fp4")) return st;
   if (x.mode != w.mode) return fail(LTXQ_ERR_INVALID, "qlinear_fp4: x and the weight have different formats");
+  if (fp4_rows_supported(M, w)) {
+    gemm::Params q = p;
+    q.alpha = gx * gw;
+    return launch_fp4_rows(nullptr, false, &x, w, q, stream);
+  }
   if (!w.mx_scales || (reinterpret_cast<uintptr_t>(w.mx_scales) & 15u))
     return fail(LTXQ_ERR_INVALID, "qlinear_fp4: mx_scales (ltxq_fp4_pack_weight_scales) is NULL or not 16-byte aligned");
   fp4::GemmArgs a{static_cast<int>((M + 127) / 128), static_cast<int>((w.n_out + 127) / 128), gx * gw};

@@ -66,22 +66,82 @@ __device__ __forceinline__ uint32_t scale_bf16x2(uint32_t s) {
   return (F == kNv ? e4m3_bf16(s) : e8m0_bf16(s)) * 0x00010001u;
 }
 
-// One packed word (elements k..k+7) times the group's scale (bf16x2
-// broadcast) -> four bf16x2 words.  A nibble s|ee|m moved to bf16 bits 15 and
-// 8:6 is the bf16 encoding of its value times 2^-126 (ee = 0 becomes a bf16
-// subnormal, as in E2M1): two products, by 2^126 (exact) and by the scale.
-// E2M1 times either scale has at most 6 significant bits, so the result is
-// exact wherever bf16's exponent range holds it.
-__device__ __forceinline__ uint32_t e2m1x2_bf16(uint32_t w, uint32_t u, int j) {
-  // byte 0 <- byte j of w (element 2j in its low nibble), byte 2 <- byte j of w >> 4
-  const uint32_t t = __byte_perm(w, u, static_cast<uint32_t>(j) | (static_cast<uint32_t>(4 + j) << 8)) & 0x000F000Fu;
-  return (t * 0x1040u) & 0x81C081C0u;  // nibble << 12 and << 6: no carries, the halves do not meet
-}
-__device__ __forceinline__ void decode_word(uint32_t w, uint32_t s2, uint32_t (&o)[4]) {
-  const uint32_t u = w >> 4;
+// A packed word holds elements k..k+7.  A nibble s|ee|m moved to bf16 bits 15
+// and 8:6 is the bf16 encoding of its value times 2^-126 (ee = 0 becomes a bf16
+// subnormal, as in E2M1), which one product with 2^126 times the scale makes
+// the value.  E2M1 times either scale has at most 6 significant bits, so the
+// product is exact wherever bf16's exponent range holds it.
+//
+// bf16x2 of (element 2j, element 2j + 1) * 2^-126 for j = 0..3; lo / hi: the
+// word's even / odd elements, one in each byte's low nibble.  The byte
+// selectors 8..F replicate a byte's top bit, here 0.
+__device__ __forceinline__ void e2m1x8_m126(uint32_t w, uint32_t (&o)[4]) {
+  const uint32_t lo = w & 0x0F0F0F0Fu, hi = (w >> 4) & 0x0F0F0F0Fu;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    o[j] = fma_bf16x2(fma_bf16x2(e2m1x2_bf16(w, u, j), 0x7E807E80u, 0x80008000u), s2, 0x80008000u);
+  for (int j = 0; j < 4; ++j) {
+    uint32_t t;
+    const uint32_t sel = static_cast<uint32_t>(j) | (8u << 4) | (static_cast<uint32_t>(4 + j) << 8) | (8u << 12);
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(t) : "r"(lo), "r"(hi), "r"(sel));
+    o[j] = (t * 0x1040u) & 0x81C081C0u;  // nibble << 12 and << 6: no carries, the halves do not meet
+  }
+}
+// times the scale (bf16x2 broadcast), any scale: 2^126 first, as its product
+// with a scale above 2 leaves bf16's range
+__device__ __forceinline__ void decode_word(uint32_t w, uint32_t s2, uint32_t (&o)[4]) {
+  e2m1x8_m126(w, o);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] = fma_bf16x2(fma_bf16x2(o[j], 0x7E807E80u, 0x80008000u), s2, 0x80008000u);
+}
+
+// The products' form, one multiplication per pair: the values times
+// kDecodeScale, by a multiplier that holds 2^126 * scale * kDecodeScale.
+//   nvfp4: 2^-8, which brings every E4M3 scale into range; the product is
+//          multiplied back with its tensor scale
+//   mxfp4: 1; scales above 2 (and the NaN code) do not fit and say so, and
+//          take decode_word
+template <int F>
+constexpr float kDecodeScale = F == kNv ? 0x1p-8f : 1.f;
+
+// the multipliers of two groups, whose scale bytes are s's low two (mxfp4: of
+// one group, its byte in s, both the same)
+template <int F>
+__device__ __forceinline__ void decode_mul2(uint32_t s, uint32_t (&m)[2], bool& fits) {
+  if (F == kNv) {
+    fits = true;
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(s)));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    // E4M3 stays below 2^9: 2^118 times it is finite in fp32, and has 4 bits, all of them in the upper half
+    const uint32_t a = __float_as_uint(__fmul_rn(f.x, 0x1p118f)), b = __float_as_uint(__fmul_rn(f.y, 0x1p118f));
+    m[0] = __byte_perm(a, a, 0x3232);
+    m[1] = __byte_perm(b, b, 0x3232);
+  } else {
+    fits = s <= 128u;
+    m[0] = m[1] = (s + 126u) * 0x00800080u;  // 2^(s - 127 + 126)
+  }
+}
+__device__ __forceinline__ void decode_word1(uint32_t w, uint32_t m2, uint32_t (&o)[4]) {
+  e2m1x8_m126(w, o);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] = fma_bf16x2(o[j], m2, 0x80008000u);
+}
+
+// decode_word1 in the order (0, 4), (1, 5), (2, 6), (3, 7), for products whose
+// other operand is laid out the same way: nibbles j and j + 4 are the two
+// halves' as they lie, so only a mask and a multiplication place them.
+__device__ __forceinline__ void decode_word1_split(uint32_t w, uint32_t m2, uint32_t (&o)[4]) {
+  const uint32_t v = w >> 8;
+  o[0] = ((w & 0x000F000Fu) * 0x1040u) & 0x81C081C0u;
+  o[1] = ((w & 0x00F000F0u) * 0x0104u) & 0x81C081C0u;
+  o[2] = ((v & 0x000F000Fu) * 0x1040u) & 0x81C081C0u;
+  o[3] = ((v & 0x00F000F0u) * 0x0104u) & 0x81C081C0u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] = fma_bf16x2(o[j], m2, 0x80008000u);
+}
+// eight bf16 values (bf16x2 words, in order) in that order
+__device__ __forceinline__ uint4 split_order(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return make_uint4(__byte_perm(a, c, 0x5410), __byte_perm(a, c, 0x7632), __byte_perm(b, d, 0x5410),
+                    __byte_perm(b, d, 0x7632));
 }
 
 // ---------------------------------------------------------------- encoding

@@ -1,8 +1,8 @@
 // gemm_epilogue.cuh -- pieces shared by the quantized GEMM kernels (qgemm.cu
 // for the dequantizing path, mx.cu for the native block-scaled fp8 path):
 // the launch parameters, the reference's GELU with its per-op bf16 rounding
-// (exact table form), named barriers and the epilogue's row store with the
-// gated residual fused.
+// (exact table form), named barriers, the epilogue's row store with the gated
+// residual fused, and the epilogue of 8 features of one token.
 #pragma once
 
 #include "common.cuh"
@@ -119,6 +119,73 @@ __device__ __forceinline__ void epi_row_store(const Params& p, uint32_t (&u)[4],
   }
   *reinterpret_cast<uint4*>(p.out + off) = make_uint4(u[0], u[1], u[2], u[3]);
 }
+
+// Epilogue state of one thread for a fixed chunk of 8 features [nf, nf + 8):
+// the linear bias and a broadcast gate are loaded once.  store() takes the
+// bf16-rounded accumulators of one token (the reference's first rounding
+// point) and applies bias / GELU / gated residual with the reference's
+// rounding points, then writes 16 bytes.
+struct Epi8 {
+  float bias8[8];
+  float g8[8];
+  bool gated, two_round, gate_bcast;
+  __device__ __forceinline__ void init(const Params& p, int nf) {
+    gated = p.epi == LTXQ_EPI_GATED_RESIDUAL || p.epi == LTXQ_EPI_GATE_THEN_ADD;
+    two_round = p.epi == LTXQ_EPI_GATE_THEN_ADD || p.gate.dtype == LTXQ_BF16;
+    gate_bcast = p.gate.rows_per_vec == 0;
+    if (p.bias != nullptr) {
+      const uint4 bv = __ldg(reinterpret_cast<const uint4*>(p.bias + nf));
+      const uint32_t bw[4] = {bv.x, bv.y, bv.z, bv.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        bias8[2 * k] = lo_bf16(bw[k]);
+        bias8[2 * k + 1] = hi_bf16(bw[k]);
+      }
+    }
+    if (gated && gate_bcast) load_vec8(p.gate, vec_row(p.gate, 0), nf, g8);
+  }
+  // conversions to bf16 are paired (cvt.rn.bf16x2.f32), never one value at a time
+  __device__ __forceinline__ void store(const Params& p, const float (&a)[8], int m, int nf, const uint16_t* gtab) {
+    uint32_t u[4];
+    if (p.bias != nullptr) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        u[k] = pack_bf16x2(__fadd_rn(a[2 * k], bias8[2 * k]), __fadd_rn(a[2 * k + 1], bias8[2 * k + 1]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) u[k] = pack_bf16x2(a[2 * k], a[2 * k + 1]);  // exact: a is bf16-valued
+    }
+    if (p.epi == LTXQ_EPI_GELU) {
+      if (gtab != nullptr) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u[k] = gelu_tab_x2(u[k], gtab);
+      } else {  // no table: the same function evaluated directly
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          u[k] = pack_bf16x2(gelu_ref(lo_bf16(u[k])), gelu_ref(hi_bf16(u[k])));
+      }
+    }
+    const int64_t off = static_cast<int64_t>(m) * p.N + nf;
+    if (gated) {
+      const uint4 rv = __ldg(reinterpret_cast<const uint4*>(p.residual + off));
+      const uint32_t rw[4] = {rv.x, rv.y, rv.z, rv.w};
+      if (!gate_bcast) load_vec8(p.gate, vec_row(p.gate, m), nf, g8);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float p0 = __fmul_rn(lo_bf16(u[k]), g8[2 * k]);
+        const float p1 = __fmul_rn(hi_bf16(u[k]), g8[2 * k + 1]);
+        const float r0 = lo_bf16(rw[k]), r1 = hi_bf16(rw[k]);
+        if (two_round) {
+          const uint32_t pr = pack_bf16x2(p0, p1);
+          u[k] = pack_bf16x2(__fadd_rn(r0, lo_bf16(pr)), __fadd_rn(r1, hi_bf16(pr)));
+        } else {
+          u[k] = pack_bf16x2(__fadd_rn(p0, r0), __fadd_rn(p1, r1));
+        }
+      }
+    }
+    *reinterpret_cast<uint4*>(p.out + off) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+};
 
 }  // namespace gemm
 

@@ -46,6 +46,9 @@ size_t mx_workspace_bytes(int64_t M, const ltxq_qweight& w);
 ltxq_status launch_qlinear_mx(const void* x, int64_t M, const ltxq_qweight& w, const gemm::Params& p, void* workspace,
                               cudaStream_t stream);
 size_t fp4_workspace_bytes(int64_t M, const ltxq_qweight& w);
+bool fp4_rows_supported(int64_t M, const ltxq_qweight& w);
+ltxq_status launch_fp4_rows(const void* x, bool quantize, const ltxq_fp4_act* packed, const ltxq_qweight& w,
+                            const gemm::Params& p, cudaStream_t stream);
 ltxq_status launch_qlinear_fp4_from_bf16(const void* x, int64_t M, const ltxq_qweight& w, const gemm::Params& p,
                                          void* workspace, cudaStream_t stream);
 ltxq_status fp4_global_scale(int32_t mode, float g, float* out, const char* what);
@@ -290,15 +293,27 @@ __device__ __forceinline__ void dequant_loop(const Params& p, const Bars& bb, ui
         // rows as for kAffine4; one scale per half (mxfp4) or per 16 elements (nvfp4)
         const uint4 v = *reinterpret_cast<const uint4*>(wrow + ((half ^ ((r >> 2) & 1)) << 4));
         const uint32_t wv[4] = {v.x, v.y, v.z, v.w};
-        uint32_t s2[2];
-        s2[0] = fp4::scale_bf16x2<QK == kNvfp4 ? fp4::kNv : fp4::kMx>(s_cur & 0xFFu);
-        s2[1] = QK == kNvfp4 ? fp4::scale_bf16x2<fp4::kNv>(s_cur >> 8) : s2[0];
+        constexpr int F = QK == kNvfp4 ? fp4::kNv : fp4::kMx;
+        bool fits;
+        uint32_t mul[2];
+        fp4::decode_mul2<F>(s_cur, mul, fits);
+        if (QK == kNvfp4 || __all_sync(0xffffffffu, fits)) {
 #pragma unroll
-        for (int w4 = 0; w4 < 4; ++w4) {
-          uint32_t q4[4];
-          fp4::decode_word(wv[w4], s2[w4 >> 1], q4);
+          for (int w4 = 0; w4 < 4; ++w4) {
+            uint32_t q4[4];
+            fp4::decode_word1(wv[w4], mul[w4 >> 1], q4);
 #pragma unroll
-          for (int t = 0; t < 4; ++t) o[w4 * 4 + t] = q4[t];
+            for (int t = 0; t < 4; ++t) o[w4 * 4 + t] = q4[t];
+          }
+        } else {
+          const uint32_t s2 = fp4::scale_bf16x2<F>(s_cur);
+#pragma unroll
+          for (int w4 = 0; w4 < 4; ++w4) {
+            uint32_t q4[4];
+            fp4::decode_word(wv[w4], s2, q4);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) o[w4 * 4 + t] = q4[t];
+          }
         }
       } else {
         // 64-byte rows, 64B swizzle: 16-byte chunk c sits at c ^ ((r >> 1) & 3);
@@ -340,9 +355,9 @@ __device__ __forceinline__ void dequant_loop(const Params& p, const Bars& bb, ui
   if (pend_as >= 0) publish(pend_as);
 }
 
-// An accumulator's value: nvfp4 weights enter as code * scale, their tensor
-// scale multiplies the fp32 sum (one product per output, and code * scale
-// stays exact in bf16).
+// An accumulator's value: nvfp4 weights enter as code * scale * kDecodeScale
+// (exact in bf16); the rest, their tensor scale among it, multiplies the fp32
+// sum, one product per output.
 template <int QK>
 __device__ __forceinline__ float scaled(const Params& p, uint32_t acc) {
   return QK == kNvfp4 ? __fmul_rn(__uint_as_float(acc), p.alpha) : __uint_as_float(acc);
@@ -575,73 +590,6 @@ struct PairPlan {
   static_assert(kStages >= 4, "pipeline depth");
   static_assert(4 * kStages * 8 + 2 * kAStages * 8 + 24 <= 512, "barrier block");
   static_assert(kSmem <= 227 * 1024, "shared memory budget");
-};
-
-// Epilogue state of one thread for a fixed chunk of 8 features [nf, nf + 8):
-// the linear bias and a broadcast gate are loaded once.  store() takes the
-// bf16-rounded accumulators of one token (the reference's first rounding
-// point) and applies bias / GELU / gated residual with the reference's
-// rounding points, then writes 16 bytes.
-struct Epi8 {
-  float bias8[8];
-  float g8[8];
-  bool gated, two_round, gate_bcast;
-  __device__ __forceinline__ void init(const Params& p, int nf) {
-    gated = p.epi == LTXQ_EPI_GATED_RESIDUAL || p.epi == LTXQ_EPI_GATE_THEN_ADD;
-    two_round = p.epi == LTXQ_EPI_GATE_THEN_ADD || p.gate.dtype == LTXQ_BF16;
-    gate_bcast = p.gate.rows_per_vec == 0;
-    if (p.bias != nullptr) {
-      const uint4 bv = __ldg(reinterpret_cast<const uint4*>(p.bias + nf));
-      const uint32_t bw[4] = {bv.x, bv.y, bv.z, bv.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        bias8[2 * k] = lo_bf16(bw[k]);
-        bias8[2 * k + 1] = hi_bf16(bw[k]);
-      }
-    }
-    if (gated && gate_bcast) load_vec8(p.gate, vec_row(p.gate, 0), nf, g8);
-  }
-  // conversions to bf16 are paired (cvt.rn.bf16x2.f32), never one value at a time
-  __device__ __forceinline__ void store(const Params& p, const float (&a)[8], int m, int nf, const uint16_t* gtab) {
-    uint32_t u[4];
-    if (p.bias != nullptr) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        u[k] = pack_bf16x2(__fadd_rn(a[2 * k], bias8[2 * k]), __fadd_rn(a[2 * k + 1], bias8[2 * k + 1]));
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) u[k] = pack_bf16x2(a[2 * k], a[2 * k + 1]);  // exact: a is bf16-valued
-    }
-    if (p.epi == LTXQ_EPI_GELU) {
-      if (gtab != nullptr) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) u[k] = gelu_tab_x2(u[k], gtab);
-      } else {  // no table: the same function evaluated directly
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          u[k] = pack_bf16x2(gelu_ref(lo_bf16(u[k])), gelu_ref(hi_bf16(u[k])));
-      }
-    }
-    const int64_t off = static_cast<int64_t>(m) * p.N + nf;
-    if (gated) {
-      const uint4 rv = __ldg(reinterpret_cast<const uint4*>(p.residual + off));
-      const uint32_t rw[4] = {rv.x, rv.y, rv.z, rv.w};
-      if (!gate_bcast) load_vec8(p.gate, vec_row(p.gate, m), nf, g8);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float p0 = __fmul_rn(lo_bf16(u[k]), g8[2 * k]);
-        const float p1 = __fmul_rn(hi_bf16(u[k]), g8[2 * k + 1]);
-        const float r0 = lo_bf16(rw[k]), r1 = hi_bf16(rw[k]);
-        if (two_round) {
-          const uint32_t pr = pack_bf16x2(p0, p1);
-          u[k] = pack_bf16x2(__fadd_rn(r0, lo_bf16(pr)), __fadd_rn(r1, hi_bf16(pr)));
-        } else {
-          u[k] = pack_bf16x2(__fadd_rn(p0, r0), __fadd_rn(p1, r1));
-        }
-      }
-    }
-    *reinterpret_cast<uint4*>(p.out + off) = make_uint4(u[0], u[1], u[2], u[3]);
-  }
 };
 
 // Split tiles: out[m, nf..nf+8) from the fp32 partial sums of a split
@@ -1603,6 +1551,8 @@ ltxq_status launch_qlinear(const void* x, int64_t M, const ltxq_qweight& w, cons
   const bool f4 = w.mode == LTXQ_MXFP4 || w.mode == LTXQ_NVFP4;
   const int64_t N = w.n_out, K = w.k_in;
 
+  // a few rows with an fp4 weight, in either compute
+  if (f4 && fp4_rows_supported(M, w)) return launch_fp4_rows(x, w.compute == LTXQ_COMPUTE_FP4, nullptr, w, p, stream);
   // products of two fp4 operands (LTXQ_COMPUTE_FP4): the workspace holds the quantized activations
   if (const size_t bytes = fp4_workspace_bytes(M, w)) {
     if (!workspace || workspace_bytes < bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u))
@@ -1622,6 +1572,7 @@ ltxq_status launch_qlinear(const void* x, int64_t M, const ltxq_qweight& w, cons
                  : w.mode == LTXQ_MXFP4 ? gemm::kMxfp4
                  : w.mode == LTXQ_NVFP4 ? gemm::kNvfp4
                                         : (w.bits == 8 ? gemm::kAffine8 : gemm::kAffine4);
+  if (w.mode == LTXQ_NVFP4) p.alpha /= fp4::kDecodeScale<fp4::kNv>;
   gemm::Sched sched = gemm::plan_schedule(M, N, K);
   if (sched.splits > 1 && (!workspace || workspace_bytes < gemm::splitk_bytes(M, N, K) ||
                            (reinterpret_cast<uintptr_t>(workspace) & 15u)))

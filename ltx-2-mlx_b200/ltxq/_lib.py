@@ -135,7 +135,7 @@ SIGNATURES = {
                                          c_void_p, c_float, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
     "ltxq_attention": (c_int32, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
                                  c_int64, c_int64, c_float, c_void_p, c_void_p]),
-    "ltxq_rotary": (c_int32, [POINTER(RotaryArgs), c_void_p]),
+    "ltxq_rotary": (c_int32, [c_void_p, c_void_p]),  # RotaryArgs, by reference or packed
     "ltxq_fp4_sizes": (c_size_t, [c_int64, c_int64, c_int32, POINTER(c_size_t), POINTER(c_size_t)]),
     "ltxq_fp4_quantize": (c_int32, [c_void_p, c_int64, c_int64, c_int64, POINTER(Fp4Act), c_void_p]),
     "ltxq_fp4_dequantize": (c_int32, [POINTER(Fp4Act), c_int64, c_int64, c_void_p, c_void_p]),

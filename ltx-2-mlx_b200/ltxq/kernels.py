@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -20,8 +21,12 @@ from . import _lib
 _DT = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 
 
+_device = torch._C._cuda_getDevice  # the current device and its current stream, without wrapping objects
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(_device())
 
 
 def _require_cuda(t: torch.Tensor, name: str) -> None:
@@ -172,6 +177,7 @@ class FP4Tensor:
             raise ValueError("global_scale is nvfp4 only")
         if not 2.0 ** -64 <= self.global_scale <= 2.0 ** 64:
             raise ValueError("global_scale must be within [2^-64, 2^64]")
+        self._st = None
         self._code_bytes = self.M * (self.K // 2)
         self._scale_bytes = -(-self.K // 256) * -(-self.M // 128) * 128 * (256 // group)
         self._scale_off = _align(self._code_bytes)
@@ -191,8 +197,10 @@ class FP4Tensor:
                 self.buffer[self._scale_off:self._scale_off + self._scale_bytes])
 
     def struct(self) -> _lib.Fp4Act:
-        base = self.buffer.data_ptr()
-        return _lib.Fp4Act(base, base + self._scale_off, FP4_MODES[self.mode], self.global_scale)
+        if self._st is None:
+            base = self.buffer.data_ptr()
+            self._st = _lib.Fp4Act(base, base + self._scale_off, FP4_MODES[self.mode], self.global_scale)
+        return self._st
 
     @classmethod
     def quantize(cls, x: torch.Tensor, mode: str = "nvfp4", global_scale: float = 1.0) -> "FP4Tensor":
@@ -202,27 +210,33 @@ class FP4Tensor:
             raise ValueError(f"x must be bfloat16, got {x.dtype}")
         if x.dim() < 1:
             raise ValueError("x must have at least one dimension")
-        with _on(x):
-            t = cls(tuple(x.shape[:-1]), x.shape[-1], mode, x.device, global_scale)
-            if t.M == 0:
-                return t
-            if x.dim() != 2 or x.stride(1) != 1 or x.stride(0) % 8 != 0 or x.stride(0) < t.K or x.data_ptr() % 16:
-                x = x.reshape(t.M, t.K)  # rows at one stride; copied where they are not
-                if x.stride(1) != 1 or x.stride(0) % 8 != 0 or x.stride(0) < t.K or x.data_ptr() % 16:
-                    x = x.clone(memory_format=torch.contiguous_format)
-            st = t.struct()
-            _lib.check(_lib.load().ltxq_fp4_quantize(x.data_ptr(), t.M, t.K, x.stride(0) if t.M > 1 else t.K,
-                                                     ctypes.byref(st), _stream()), "fp4_quantize")
+        dev = x.get_device()
+        if dev != _device():
+            with torch.cuda.device(dev):
+                return cls.quantize(x, mode, global_scale)
+        t = cls(x.shape[:-1], x.shape[-1], mode, x.device, global_scale)
+        if t.M == 0:
+            return t
+        stride = t.K
+        if not x.is_contiguous() or x.data_ptr() % 16:
+            x = x.reshape(t.M, t.K)  # rows at one stride; copied where they are not
+            if x.stride(1) != 1 or x.stride(0) % 8 != 0 or x.stride(0) < t.K or x.data_ptr() % 16:
+                x = x.clone(memory_format=torch.contiguous_format)
+            stride = x.stride(0) if t.M > 1 else t.K
+        _lib.check(_lib.load().ltxq_fp4_quantize(x.data_ptr(), t.M, t.K, stride, t.struct(), _raw_stream(dev)),
+                   "fp4_quantize")
         return t
 
     def dequantize(self) -> torch.Tensor:
         """The values, as bf16 of the quantized tensor's shape."""
-        with _on(self.buffer):
-            out = torch.empty(self.shape, dtype=torch.bfloat16, device=self.device)
-            if self.M:
-                st = self.struct()
-                _lib.check(_lib.load().ltxq_fp4_dequantize(ctypes.byref(st), self.M, self.K, out.data_ptr(), _stream()),
-                           "fp4_dequantize")
+        dev = self.buffer.get_device()
+        if dev != _device():
+            with torch.cuda.device(dev):
+                return self.dequantize()
+        out = torch.empty(self.shape, dtype=torch.bfloat16, device=self.buffer.device)
+        if self.M:
+            _lib.check(_lib.load().ltxq_fp4_dequantize(self.struct(), self.M, self.K, out.data_ptr(), _raw_stream(dev)),
+                       "fp4_dequantize")
         return out
 
 
@@ -431,6 +445,7 @@ def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, heads: int, eps: float =
 
 
 _POS = {torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64, torch.float32: _lib.POS_F32, torch.float64: _lib.POS_F64}
+_ROTARY_ARGS = struct.Struct("@PPii5q3q3qP3qiiPPiifi")  # _lib.RotaryArgs
 _ROTARY_LAYOUT = {"half": _lib.ROTARY_HALF, "interleaved": _lib.ROTARY_INTERLEAVED}
 
 
@@ -487,31 +502,32 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, heads:
         axes = axes.contiguous()
         if n_axes < 1:
             raise ValueError("positions have no axis")
-    for o, name in ((positions, "positions"), (freqs, "freqs"), (axes, "axes"), (out, "out")):
-        if o is not None and o.device != x.device:
-            raise ValueError(f"{name} is on {o.device}, x on {x.device}")
+    dev = x.get_device()
+    if positions.get_device() != dev or freqs.get_device() != dev or (axes is not None and axes.get_device() != dev) or (
+            out is not None and out.get_device() != dev):
+        raise ValueError(f"positions, freqs, axes and out must be on x's device ({x.device})")
     if d == 0:
         raise ValueError("heads have no elements")
-    with _on(x):
-        if x.stride(-1) != 1 and x.shape[-1] > 1:
-            if out is x:
-                raise ValueError("an in-place rotation needs x with a unit last stride")
-            x = x.contiguous()
-        if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        elif out.shape != x.shape or out.dtype != x.dtype or (out.stride(-1) != 1 and out.shape[-1] > 1):
-            raise ValueError("out must have x's shape and type and a unit last stride")
-        if x.numel() == 0:
-            return out
-        freqs = freqs.contiguous()
-        st = _lib.RotaryArgs(x=x.data_ptr(), out=out.data_ptr(), dtype=_DT[x.dtype], layout=_ROTARY_LAYOUT[layout],
-                             batch=b, tokens=t, heads=heads, head_dim=d, rotary_dim=r,
-                             positions=positions.data_ptr(), pos_dtype=_POS[positions.dtype], n_axes=n_axes,
-                             freqs=freqs.data_ptr(), axis=axes.data_ptr() if axes is not None else None,
-                             freqs_per_head=int(freqs.dim() == 2), inverse=int(bool(inverse)), scale=float(scale))
-        st.x_stride[:] = (x.stride(0), x.stride(1), x.stride(2) if x.dim() == 4 else d)
-        st.out_stride[:] = (out.stride(0), out.stride(1), out.stride(2) if out.dim() == 4 else d)
-        st.pos_stride[:] = (positions.stride(0) if lead else 0, positions.stride(-2) if axes is not None else 0,
-                            positions.stride(-1))
-        _lib.check(_lib.load().ltxq_rotary(ctypes.byref(st), _stream()), "rotary")
+    if dev != _device():
+        with torch.cuda.device(dev):
+            return rotary(x, positions, freqs, heads, layout=layout, axes=axes, scale=scale, inverse=inverse, out=out)
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        if out is x:
+            raise ValueError("an in-place rotation needs x with a unit last stride")
+        x = x.contiguous()
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or (out.stride(-1) != 1 and out.shape[-1] > 1):
+        raise ValueError("out must have x's shape and type and a unit last stride")
+    if x.numel() == 0:
+        return out
+    freqs = freqs.contiguous()
+    xs, os, ps = x.stride(), out.stride(), positions.stride()
+    four = len(xs) == 4
+    args = _ROTARY_ARGS.pack(
+        x.data_ptr(), out.data_ptr(), _DT[x.dtype], _ROTARY_LAYOUT[layout], b, t, heads, d, r, xs[0], xs[1],
+        xs[2] if four else d, os[0], os[1], os[2] if four else d, positions.data_ptr(), ps[0] if lead else 0,
+        ps[-2] if axes is not None else 0, ps[-1], _POS[positions.dtype], n_axes, freqs.data_ptr(),
+        axes.data_ptr() if axes is not None else 0, freqs.dim() == 2, bool(inverse), scale, 0)
+    _lib.check(_lib.load().ltxq_rotary(args, _raw_stream(dev)), "rotary")
     return out

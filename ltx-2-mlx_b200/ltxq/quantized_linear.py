@@ -23,7 +23,8 @@ import math
 import torch
 
 from . import _lib
-from .kernels import FP4_MODES, FP4Tensor, MXActivation, _on, _require_cuda, _stream, prologue, vec_arg
+from .kernels import (FP4_MODES, FP4Tensor, MXActivation, _device, _on, _raw_stream, _require_cuda, _stream, prologue,
+                      vec_arg)
 
 QUANT_DEFAULTS = {"affine": (64, 4), "mxfp8": (32, 8), "mxfp4": (32, 4), "nvfp4": (16, 4)}
 _MODE = {"affine": _lib.AFFINE, "mxfp8": _lib.MXFP8, **FP4_MODES}
@@ -34,6 +35,11 @@ _MODE = {"affine": _lib.AFFINE, "mxfp8": _lib.MXFP8, **FP4_MODES}
 # to the weight's format)
 COMPUTE = {"dequant": _lib.COMPUTE_DEQUANT, "mx2": _lib.COMPUTE_MX2, "mx1": _lib.COMPUTE_MX1,
            "fp4": _lib.COMPUTE_FP4}
+
+
+def _version(t: torch.Tensor) -> int:
+    """torch's in-place version counter (tensors made in inference mode have none)."""
+    return 0 if t.is_inference() else t._version
 
 
 def quant_defaults(mode: str, group_size: int | None, bits: int | None) -> tuple[int, int]:
@@ -97,7 +103,7 @@ class QuantizedLinear:
         (``ltxq_fp4_pack_weight_scales``), made once and again only when the
         scale tensor changes; None where those modes do not apply."""
         if self.computes_fp4():
-            key = (self.scales.data_ptr(), self.scales._version)
+            key = (self.scales.data_ptr(), _version(self.scales))
             cached = getattr(self, "_mx_scales", None)
             if cached is None or cached[0] != key:
                 with _on(self.scales):
@@ -264,19 +270,10 @@ class QuantizedLinear:
 
         With compute "fp4" on an mxfp4 / nvfp4 weight, ``x`` is quantized to
         the weight's format in the call, or comes as an ``FP4Tensor`` of it."""
-        if isinstance(x, FP4Tensor) or self.mode in FP4_MODES:
+        if self.mode in FP4_MODES or isinstance(x, FP4Tensor):
             if mx_out:
                 raise ValueError("mx_out needs an MXActivation input (the block-scaled fp8 kernels)")
-            dev = x.device
-            if dev != self.weight.device:
-                raise ValueError(f"x is on {dev}, the weight on {self.weight.device}")
-            if isinstance(x, FP4Tensor):
-                with _on(self.weight):
-                    return self._call_fp4(x, gelu, residual, gate, gate_then_add, adaln)
-            if dev.index != torch.cuda.current_device() and dev.type == "cuda":
-                with _on(self.weight):
-                    return self(x, gelu=gelu, residual=residual, gate=gate, gate_then_add=gate_then_add, adaln=adaln,
-                                split_k=split_k)
+            return self._call_fp4(x, gelu, residual, gate, gate_then_add, adaln, split_k)
         if isinstance(x, MXActivation):
             return self._call_mx(x, gelu, residual, gate, gate_then_add, mx_out)
         if mx_out:
@@ -292,8 +289,6 @@ class QuantizedLinear:
         keep: list = []
         epi = self._epilogue(rows_shape, keep, gelu, residual, gate, gate_then_add)
         out = torch.empty(rows_shape + (self.out_features,), dtype=torch.bfloat16, device=x.device)
-        if M == 0:
-            return out
         q = self.qweight()
         lib = _lib.load()
         if adaln is not None:
@@ -306,28 +301,78 @@ class QuantizedLinear:
             _lib.check(lib.ltxq_adaln_qlinear(x.data_ptr(), M, ctypes.byref(pro), ctypes.byref(q), ctypes.byref(epi),
                                               out.data_ptr(), ws.data_ptr(), ws_bytes, _stream()), "adaln_qlinear")
         else:
-            ws_bytes = (lib.ltxq_qlinear_workspace_size(M, ctypes.byref(q)) if split_k or self.computes_fp4() else 0)
+            ws_bytes = lib.ltxq_qlinear_workspace_size(M, ctypes.byref(q)) if split_k else 0
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
             _lib.check(lib.ltxq_qlinear(x.data_ptr(), M, ctypes.byref(q), ctypes.byref(epi), out.data_ptr(),
                                         ws.data_ptr() if ws is not None else None, ws_bytes, _stream()), "qlinear")
         return out
 
-    def _call_fp4(self, x: FP4Tensor, gelu, residual, gate, gate_then_add, adaln):
-        if not self.computes_fp4() or x.mode != self.mode:
-            raise ValueError(f"an {x.mode} input needs an {x.mode} weight whose compute is 'fp4' (weight: {self.mode}, "
-                             f"compute: {self.compute})")
-        if adaln is not None:
-            raise ValueError("adaln takes bf16 activations")
-        if x.K != self.in_features:
-            raise ValueError(f"x last dim {x.K} != in_features {self.in_features}")
-        keep: list = []
-        epi = self._epilogue(x.rows_shape, keep, gelu, residual, gate, gate_then_add)
-        out = torch.empty(x.rows_shape + (self.out_features,), dtype=torch.bfloat16, device=x.device)
-        if x.M == 0:
+    def _qweight4(self) -> _lib.QWeight:
+        """``qweight()`` of an fp4 weight, kept until one of its tensors or
+        settings changes."""
+        key = (self.weight.data_ptr(), self.scales.data_ptr(), _version(self.scales),
+               self.bias.data_ptr() if self.bias is not None else 0, self.compute, self.global_scale)
+        cached = getattr(self, "_q4", None)
+        if cached is None or cached[0] != key:
+            cached = (key, self.qweight())
+            self._q4 = cached
+        return cached[1]
+
+    def _call_fp4(self, x, gelu, residual, gate, gate_then_add, adaln, split_k):
+        """Products over an mxfp4 / nvfp4 weight, from bf16 rows or an ``FP4Tensor``."""
+        packed = isinstance(x, FP4Tensor)
+        if packed:
+            if not self.computes_fp4() or x.mode != self.mode:
+                raise ValueError(f"an {x.mode} input needs an {x.mode} weight whose compute is 'fp4' (weight: "
+                                 f"{self.mode}, compute: {self.compute})")
+            if adaln is not None:
+                raise ValueError("adaln takes bf16 activations")
+            device = x.buffer.device
+        else:
+            if isinstance(x, MXActivation):
+                raise ValueError("an MXActivation input needs an mxfp8 weight")
+            _require_cuda(x, "x")
+            if x.dtype != torch.bfloat16:
+                raise ValueError(f"x must be bfloat16, got {x.dtype}")
+            device = x.device
+        dev = self.weight.get_device()
+        if device.index != dev:
+            raise ValueError(f"x is on {device}, the weight on {self.weight.device}")
+        if x.shape[-1] != self.in_features:
+            raise ValueError(f"x last dim {x.shape[-1]} != in_features {self.in_features}")
+        if dev != _device():
+            with torch.cuda.device(dev):
+                return self._call_fp4(x, gelu, residual, gate, gate_then_add, adaln, split_k)
+        rows_shape = x.shape[:-1]
+        out = torch.empty((*rows_shape, self.out_features), dtype=torch.bfloat16, device=device)
+        M = x.M if packed else x.numel() // self.in_features
+        if M == 0:
             return out
-        q, xs = self.qweight(), x.struct()
-        _lib.check(_lib.load().ltxq_qlinear_fp4(ctypes.byref(xs), x.M, ctypes.byref(q), ctypes.byref(epi),
-                                                out.data_ptr(), _stream()), "qlinear_fp4")
+        keep: list = []
+        epi = None  # no epilogue
+        if gelu or residual is not None:
+            epi = self._epilogue(tuple(rows_shape), keep, gelu, residual, gate, gate_then_add)
+        q, lib, stream = self._qweight4(), _lib.load(), _raw_stream(dev)
+        if packed:
+            _lib.check(lib.ltxq_qlinear_fp4(x.struct(), M, q, epi, out.data_ptr(), stream), "qlinear_fp4")
+            return out
+        if not x.is_contiguous() or x.data_ptr() % 16:
+            x = x.clone(memory_format=torch.contiguous_format)
+        pro = None
+        if adaln is not None:
+            norm = {"rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER, "none": _lib.NORM_NONE}[
+                adaln[3] if len(adaln) > 3 else "rms"]
+            pro = prologue(norm, adaln[2], adaln[0], adaln[1], tuple(rows_shape), self.in_features, keep)
+            ws_bytes = lib.ltxq_adaln_qlinear_workspace_size(M, q)
+        else:
+            ws_bytes = lib.ltxq_qlinear_workspace_size(M, q) if split_k or self.compute == "fp4" else 0
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
+        ws_ptr = ws.data_ptr() if ws is not None else None
+        if pro is not None:
+            _lib.check(lib.ltxq_adaln_qlinear(x.data_ptr(), M, pro, q, epi, out.data_ptr(), ws_ptr, ws_bytes, stream),
+                       "adaln_qlinear")
+        else:
+            _lib.check(lib.ltxq_qlinear(x.data_ptr(), M, q, epi, out.data_ptr(), ws_ptr, ws_bytes, stream), "qlinear")
         return out
 
     def _call_mx(self, x: MXActivation, gelu, residual, gate, gate_then_add, mx_out):

@@ -350,20 +350,96 @@ def test_product_refusals(cuda):
     assert lin(x, split_k=False).shape == (4, 64)
 
 
-def test_allocation_free_entry_refuses_fp4_compute(cuda):
-    """It has no workspace for quantized activations: an error, no launch of the product."""
+def test_allocation_free_entry_and_fp4_compute(cuda):
+    """It has no workspace for quantized activations: a few rows, which need none, run; more are an error."""
     import ctypes
 
     from ltxq import _lib
 
     lin, _ = _weight(rng(4), 64, 64, "nvfp4")
     lin.set_compute("fp4")
-    x = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
+    x = torch.randn(40, 64, device="cuda").bfloat16()
+    out = torch.zeros(40, 64, dtype=torch.bfloat16, device="cuda")
     z = torch.zeros(64, device="cuda")
     v = _lib.Vec(z.data_ptr(), _lib.F32, 0, 0, 0)
     q = lin.qweight()
-    st = _lib.load().ltxq_adaln_qlinear_noalloc(x.data_ptr(), 4, ctypes.byref(_lib.Prologue(_lib.NORM_RMS, 1e-6, v, v)),
-                                                ctypes.byref(q), None, x.data_ptr(), None)
-    assert st == _lib.ERR_INVALID
+    call = lambda m: _lib.load().ltxq_adaln_qlinear_noalloc(  # noqa: E731
+        x.data_ptr(), m, ctypes.byref(_lib.Prologue(_lib.NORM_RMS, 1e-6, v, v)), ctypes.byref(q), None, out.data_ptr(), None)
     torch.cuda.synchronize()
+    assert call(40) == _lib.ERR_INVALID
+    torch.cuda.synchronize()
+    assert (out == 0).all()
+    assert call(4) == _lib.OK
+    torch.cuda.synchronize()
+    assert torch.equal(out[:4], lin(x[:4], adaln=(z, z, 1e-6))) and (out[4:] == 0).all()
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("m,n,k", [(1, 16384, 4096), (4, 40, 16384), (7, 2408, 2080), (8, 4096, 8192), (16, 2048, 4096),
+                                   (12, 1000, 4064), (16, 8, 32), (3, 3000, 96)])
+def test_few_rows(cuda, mode, m, n, k):
+    """Single tokens and short batches over every number of feature tiles and K blocks, from bf16 rows, quantized in
+    the call and quantized before it."""
+    import ltxq
+
+    g = rng(m + n + k)
+    lin, w = _weight(g, n, k, mode, 1.0 if mode == "mxfp4" else 0.0156)
+    x = _values(g, (m, k))
+    _check(lin(_bf16(x)), x.astype(np.float64), w, k)
+    lin.set_compute("fp4")
+    xq = of.dequantize(*of.quantize(x, mode), mode)
+    out = lin(_bf16(x))
+    _check(out, xq, w, k)
+    assert torch.equal(lin(ltxq.FP4Tensor.quantize(_bf16(x), mode)), out)
+
+
+@pytest.mark.parametrize("m", [2, 40, 300])
+def test_large_mxfp4_scales(cuda, m):
+    """Scales above 2 leave the one-multiplication decoding: groups of every size beside one another."""
+    g = rng(m)
+    n, k = 264, 512
+    codes = g.integers(0, 16, (n, k)).astype(np.uint8)
+    scales = g.choice(np.array([0, 1, 100, 127, 128, 129, 140, 200], np.uint8), (n, k // 32))
+    scales[:64] = 127
+    import ltxq
+
+    lin = ltxq.QuantizedLinear(torch.from_numpy(of.pack(codes)).cuda().view(torch.uint32), torch.from_numpy(scales).cuda(),
+                               group_size=32, bits=4, mode="mxfp4")
+    x = _values(g, (m, k))
+    _check(lin(_bf16(x)), x.astype(np.float64), of.dequantize(codes, scales, "mxfp4"), k)
+
+
+def test_weights_made_in_inference_mode(cuda):
+    import ltxq
+
+    with torch.inference_mode():
+        w = torch.randn(64, 64, device="cuda").bfloat16()
+        lin = ltxq.QuantizedLinear.from_linear(w, mode="nvfp4").set_compute("fp4")
+        x = torch.randn(40, 64, device="cuda").bfloat16()
+        assert torch.equal(lin(x), lin(ltxq.FP4Tensor.quantize(x, "nvfp4")))
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("m,n,k", [(1, 5000, 512), (3, 2600, 4064), (16, 40, 1056)])
+def test_few_rows_of_any_range(cuda, mode, m, n, k):
+    """Rows whose values span all of bf16: none is lost beside one many binades larger, whatever the weight has there."""
+    g = rng(n)
+    lin, w = _weight(g, n, k, mode)
+    x = _values(g, (m, k)) * np.exp2(g.integers(-60, 60, (m, k))).astype(np.float32)
+    x[:, 0] = 2.0 ** 100  # alone decides the result, except where the weight is zero
+    x[0, 1:k // 2] = 0.0
+    x[m - 1, 5] = 2.0 ** -130
+    lin.scales[: n // 2, 0] = 0 if mode == "nvfp4" else 104  # (almost) nothing of the largest value
+    sc = lin.scales.cpu().numpy()
+    w = of.dequantize(of.unpack(lin.weight.cpu().view(torch.uint8).numpy()), sc, mode)
+    out = lin(_bf16(x))
+    exact = x.astype(np.float64) @ w.T
+    size = np.abs(x).astype(np.float64) @ np.abs(w).T
+    err = np.abs(from_dev_bf16(out).astype(np.float64) - exact)
+    assert (err <= 2.0 ** -8 * np.abs(exact) + k * 2.0 ** -23 * size + 2.0 ** -126).all()
+    # a row with an infinity: where its weight is not zero, infinite or NaN; the other rows as they were
+    x[0, 3] = np.inf
+    again = from_dev_bf16(lin(_bf16(x)))
+    assert np.array_equal(again[1:], from_dev_bf16(out)[1:])
+    assert (~np.isfinite(again[0][w[:, 3] != 0])).all()
