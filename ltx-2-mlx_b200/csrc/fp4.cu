@@ -185,13 +185,20 @@ namespace fp4 {
 
 // Persistent kernel, clusters of two CTAs (tcgen05 cta_group::2).  A tile is
 // 256 kBlocks tokens x 192 features: CTA r holds kBlocks blocks of 128 token
-// rows (operand A, TMEM lanes = tokens) and 96 weight rows (operand B).  Every
-// operand of a 256-K stage -- codes in the 128-byte swizzle, scale atoms as
-// they are -- arrives by TMA on one barrier of the leader, whose MMA thread
-// copies the scales to TMEM (tcgen05.cp) and issues 4 MMAs of K = 64 for each
-// block.  With tokens on the lanes an epilogue thread holds 32 consecutive
-// features of one row: bias, GELU and the gated residual need no transpose,
-// and 64 contiguous bytes of each row are written.
+// rows (operand A, TMEM lanes = tokens) and 96 weight rows (operand B).  Codes
+// of a 256-K stage (128-byte swizzle) arrive by TMA on one barrier of the
+// leader, scale atoms on one of each CTA's own.  With tokens on the lanes an
+// epilogue thread holds 32 consecutive features of one row: bias, GELU and the
+// gated residual need no transpose, and 64 contiguous bytes of each row are
+// written.
+//
+// The MMA reads its scales from tensor memory: of rows m and 32 + m, 64 + m,
+// 96 + m on lane m, the same in all four lane quarters.  Four warps per CTA,
+// one per quarter, move them there through registers (tcgen05.st), one stage
+// ahead in the other of two buffers, while the MMAs of a stage run.  Copying
+// them with tcgen05.cp from the MMA's thread instead takes the tensor pipe's
+// own time, 54 cycles an atom: at 9216 x 16384 x 4096 nvfp4 the MMAs alone took
+// 213 us, the copies alone 190 more, and the kernel 414.
 constexpr int BM = 128;       // tokens per block and CTA (MMA M = 256 for the pair)
 constexpr int BN = 192;       // features per tile (MMA N)
 constexpr int BNC = BN / 2;   // weight rows per CTA
@@ -207,10 +214,11 @@ struct Plan {
   static constexpr int kSfa = kBlocks * AP * kAtom;   // its tokens' scales
   static constexpr int kSfb = 2 * AP * kAtom;         // the two 128-feature row tiles that 192 features touch
   static constexpr int kStage = kA + kB + kSfa + kSfb;
-  static constexpr uint32_t kStageTx = 2u * kStage;   // both CTAs' bytes land on the leader's barrier
+  static constexpr uint32_t kStageTx = 2u * (kA + kB);  // both CTAs' codes land on the leader's barrier
   static constexpr int kEpiWarps = 4 * kBlocks;
-  static constexpr int kThreads = 32 * (kEpiWarps + 2);
-  static constexpr int kTmaWarp = kEpiWarps, kMmaWarp = kEpiWarps + 1;
+  static constexpr int kSfWarp0 = kEpiWarps;  // four warps that bring scales to TMEM
+  static constexpr int kTmaWarp = kEpiWarps + 4, kMmaWarp = kEpiWarps + 5;
+  static constexpr int kThreads = 32 * (kEpiWarps + 6);
   static constexpr int kAccBufs = kBlocks == 1 ? 2 : 1;
   static constexpr int kStagesRaw = (227 * 1024 - 1024 - 512 - gemm::kGeluTabBytes) / kStage;
   static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
@@ -220,26 +228,17 @@ struct Plan {
   static constexpr int kBarOff = kSfbOff + kStages * kSfb;
   static constexpr int kTabOff = kBarOff + 512;
   static constexpr int kSmem = 1024 + kTabOff + gemm::kGeluTabBytes;
-  // TMEM: accumulators, then scales: block b, atom a at kSfaCol + 4 (b AP + a); the
-  // weight's two row tiles of atom a side by side at kSfbCol + 8 a
-  static constexpr uint32_t kSfaCol = 2 * BN;
-  static constexpr uint32_t kSfbCol = kSfaCol + 4 * kBlocks * AP;
-  static_assert(kSfbCol + 8 * AP <= kTmemCols, "TMEM columns");
+  // TMEM: accumulators, then two buffers of scales: block b, atom a at 4 (b AP + a);
+  // behind them the weight's two row tiles of atom a side by side at 8 a
+  static constexpr uint32_t kSfCol = 2 * BN;
+  static constexpr uint32_t kSfbOffCol = 4 * kBlocks * AP;
+  static constexpr uint32_t kSfCols = (kSfbOffCol + 8 * AP + 15) / 16 * 16;  // stores are 16 columns wide
+  static_assert(kSfCol + 2 * kSfCols <= kTmemCols, "TMEM columns");
   static_assert(kStages >= 4, "pipeline depth");
   static_assert(kSmem <= 227 * 1024, "shared memory budget");
   static_assert(kA % 1024 == 0 && kB % 1024 == 0, "128B-swizzle atoms need 1024-byte alignment");
-  static_assert((2 * kStages + 4) * 8 + 8 <= 512, "barrier area");
+  static_assert((3 * kStages + 8) * 8 + 8 <= 512, "barrier area");
 };
-
-// Shared-memory descriptor of a scale atom for tcgen05.cp: K-major, no
-// swizzle, 32 rows of 16 bytes (8-row core matrices 128 bytes apart).
-__device__ __forceinline__ uint64_t sf_desc(uint32_t smem_addr) {
-  return static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128u >> 4) << 32) |
-         (static_cast<uint64_t>(1u) << 46);
-}
-__device__ __forceinline__ void sf_copy_pair(uint32_t taddr, uint64_t sdesc) {
-  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
-}
 
 // Instruction descriptor of kind::mxf4 / kind::mxf4nvf4: E2M1 A and B, K-major,
 // fp32 accumulators; scales E8M0 (two bytes of a scale word per MMA, sf_id 0
@@ -286,11 +285,14 @@ __global__ void __launch_bounds__(Plan<F, kBlocks>::kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + P::kBarOff);
-  uint64_t* full = bars;                   // leader: every operand of the stage landed in both CTAs
+  uint64_t* full = bars;                   // leader: the stage's codes landed in both CTAs
   uint64_t* empty = bars + S;              // stage consumed by the MMAs (commit, to both CTAs)
-  uint64_t* acc_full = bars + 2 * S;       // [kAccBufs]
-  uint64_t* acc_empty = bars + 2 * S + 2;  // [kAccBufs], leader: both CTAs' epilogues have read the accumulator
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 4);
+  uint64_t* sf_full = bars + 2 * S;        // this CTA's scales of the stage landed
+  uint64_t* acc_full = bars + 3 * S;       // [kAccBufs]
+  uint64_t* acc_empty = bars + 3 * S + 2;  // [kAccBufs], leader: both CTAs' epilogues have read the accumulator
+  uint64_t* sf_ready = bars + 3 * S + 4;   // [2], leader: both CTAs' scales are in TMEM
+  uint64_t* sf_empty = bars + 3 * S + 6;   // [2] scales in TMEM consumed (commit, to both CTAs)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * S + 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint16_t* gtab = reinterpret_cast<uint16_t*>(smem + P::kTabOff);
 
@@ -319,10 +321,15 @@ __global__ void __launch_bounds__(Plan<F, kBlocks>::kThreads, 1)
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+      mbar_init(&sf_full[s], 1);
     }
     for (int b = 0; b < P::kAccBufs; ++b) {
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 2);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sf_ready[b], 8);  // four warps of each CTA
+      mbar_init(&sf_empty[b], 1);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -337,6 +344,7 @@ __global__ void __launch_bounds__(Plan<F, kBlocks>::kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   const uint32_t leader_full = mapa_shared(smem_u32(full), 0);
   const uint32_t leader_acc_empty = mapa_shared(smem_u32(acc_empty), 0);
+  const uint32_t leader_sf_ready = mapa_shared(smem_u32(sf_ready), 0);
 
   if (warp == P::kTmaWarp) {
     if (lane == 0) {
@@ -359,8 +367,9 @@ __global__ void __launch_bounds__(Plan<F, kBlocks>::kThreads, 1)
           const uint32_t bar = leader_full + 8u * s;
           tma_load_2d_pair(smem + s * P::kA, &tmap_x, bar, kb * BKB, m0);
           tma_load_2d_pair(smem + P::kBOff + s * P::kB, &tmap_w, bar, kb * BKB, n0 + static_cast<int>(rank) * BNC);
-          tma_load_2d_pair(smem + P::kSfaOff + s * P::kSfa, &tmap_sfx, bar, 0, (kb * a.x_tiles + m0 / BM) * AP);
-          tma_load_2d_pair(smem + P::kSfbOff + s * P::kSfb, &tmap_sfw, bar, 0, (kb * a.w_tiles + n0 / 128) * AP);
+          mbar_arrive_expect_tx(&sf_full[s], P::kSfa + P::kSfb);
+          tma_load_2d(smem + P::kSfaOff + s * P::kSfa, &tmap_sfx, &sf_full[s], 0, (kb * a.x_tiles + m0 / BM) * AP);
+          tma_load_2d(smem + P::kSfbOff + s * P::kSfb, &tmap_sfw, &sf_full[s], 0, (kb * a.w_tiles + n0 / 128) * AP);
         }
       }
       if (*abort_flag) {
@@ -383,20 +392,14 @@ __global__ void __launch_bounds__(Plan<F, kBlocks>::kThreads, 1)
         const uint32_t skip = (n0 & 127) ? 2u : 0u;  // a tile that starts 64 features into a row tile
         for (int kb = 0; kb < num_kb; ++kb, ++g) {
           const int s = g % S;
-          if (!mbar_wait(&full[s], (g / S) & 1, abort_flag, p.err)) {
+          const int sb = g & 1;
+          if (!mbar_wait(&full[s], (g / S) & 1, abort_flag, p.err) ||
+              !mbar_wait(&sf_ready[sb], (g >> 1) & 1, abort_flag, p.err)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sfa_s = smem_u32(smem + P::kSfaOff + s * P::kSfa);
-          const uint32_t sfb_s = smem_u32(smem + P::kSfbOff + s * P::kSfb);
-#pragma unroll
-          for (int i = 0; i < kBlocks * AP; ++i) sf_copy_pair(tmem + P::kSfaCol + 4u * i, sf_desc(sfa_s + i * kAtom));
-#pragma unroll
-          for (int i = 0; i < AP; ++i) {
-            sf_copy_pair(tmem + P::kSfbCol + 8u * i, sf_desc(sfb_s + i * kAtom));
-            sf_copy_pair(tmem + P::kSfbCol + 8u * i + 4u, sf_desc(sfb_s + (AP + i) * kAtom));
-          }
+          const uint32_t sf = tmem + P::kSfCol + static_cast<uint32_t>(sb) * P::kSfCols;
           const uint32_t aaddr = smem_u32(smem + s * P::kA);
           const uint32_t baddr = smem_u32(smem + P::kBOff + s * P::kB);
 #pragma unroll
@@ -404,16 +407,17 @@ __global__ void __launch_bounds__(Plan<F, kBlocks>::kThreads, 1)
             const int atom = F == kNv ? kk : kk >> 1;
             const uint32_t id = F == kNv ? 0u : 2u * (kk & 1);
             const uint32_t idesc = idesc_fp4<F>(2 * BM, BN, id);
-            const uint32_t sfb = (id << 30) | (tmem + P::kSfbCol + 8u * atom + skip);
+            const uint32_t sfb = (id << 30) | (sf + P::kSfbOffCol + 8u * atom + skip);
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
               const uint32_t d = tmem + static_cast<uint32_t>((kBlocks == 1 ? buf : b) * BN);
-              const uint32_t sfa = (id << 30) | (tmem + P::kSfaCol + 4u * (b * AP + atom));
+              const uint32_t sfa = (id << 30) | (sf + 4u * (b * AP + atom));
               mma_fp4_pair<F>(d, smem_desc_sw128(aaddr + b * (BM * BKB) + kk * 32), smem_desc_sw128(baddr + kk * 32),
                               idesc, sfa, sfb, (kb | kk) != 0 ? 1u : 0u);
             }
           }
           mma_commit_pair(&empty[s], 0x3);
+          mma_commit_pair(&sf_empty[sb], 0x3);
         }
         if (!ok) break;
         mma_commit_pair(&acc_full[buf], 0x3);
@@ -423,6 +427,47 @@ __global__ void __launch_bounds__(Plan<F, kBlocks>::kThreads, 1)
         const uint64_t t0 = globaltimer();
         while (globaltimer() - t0 < 50000ull) {
         }
+      }
+    }
+  } else if (warp >= P::kSfWarp0) {
+    // ------------------------------------------------ scales, shared memory -> this warp's lane quarter of TMEM
+    const uint32_t t_lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    bool ok = true;
+    int g = 0;
+    for (int t = cluster_id; t < tiles && ok; t += n_clusters) {
+      for (int kb = 0; kb < num_kb; ++kb, ++g) {
+        const int s = g % S, sb = g & 1;
+        if (!mbar_wait(&sf_full[s], (g / S) & 1, abort_flag, p.err)) {
+          ok = false;
+          break;
+        }
+        // an atom is 32 rows of 16 bytes: a lane's row is its four columns
+        const uint8_t* sfa = smem + P::kSfaOff + s * P::kSfa + lane * 16;
+        const uint8_t* sfb = smem + P::kSfbOff + s * P::kSfb + lane * 16;
+        uint32_t r[P::kSfCols] = {};
+#pragma unroll
+        for (int i = 0; i < kBlocks * AP; ++i) {
+          const uint4 v = *reinterpret_cast<const uint4*>(sfa + i * kAtom);
+          r[4 * i] = v.x; r[4 * i + 1] = v.y; r[4 * i + 2] = v.z; r[4 * i + 3] = v.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * AP; ++i) {  // row tile i / AP, atom i % AP
+          const uint4 v = *reinterpret_cast<const uint4*>(sfb + i * kAtom);
+          const int c = P::kSfbOffCol + 8 * (i % AP) + 4 * (i / AP);
+          r[c] = v.x; r[c + 1] = v.y; r[c + 2] = v.z; r[c + 3] = v.w;
+        }
+        if (!mbar_wait(&sf_empty[sb], ((g >> 1) & 1) ^ 1, abort_flag, p.err)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t dst = tmem + t_lane + P::kSfCol + static_cast<uint32_t>(sb) * P::kSfCols;
+#pragma unroll
+        for (uint32_t c = 0; c < P::kSfCols; c += 16) tmem_st_32x32b_x16(dst + c, r + c);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(leader_sf_ready + 8u * static_cast<uint32_t>(sb));
       }
     }
   } else {
@@ -436,7 +481,6 @@ __global__ void __launch_bounds__(Plan<F, kBlocks>::kThreads, 1)
       gemm::gelu_tab_fill(gtab, threadIdx.x, 32 * P::kEpiWarps);  // while the first tile's main loop runs
       gemm::named_bar_sync(1, 32 * P::kEpiWarps);
     }
-    const float zero8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int t = cluster_id, it = 0; t < tiles; t += n_clusters, ++it) {
       int m0, n0;
       coords(t, m0, n0);
@@ -451,31 +495,7 @@ __global__ void __launch_bounds__(Plan<F, kBlocks>::kThreads, 1)
         uint32_t v[32];
         tmem_ld_32x32b_x32(tacc + c * 32, v);
         tmem_wait_ld();
-#pragma unroll
-        for (int k8 = 0; k8 < 4; ++k8) {
-          const int nf = n0 + c * 32 + k8 * 8;
-          if (nf >= p.N) break;  // uniform
-          uint32_t u[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            // bf16(x W^T) is the first rounding point, as on the dequantizing path
-            const float a0 = __fmul_rn(__uint_as_float(v[k8 * 8 + 2 * j]), a.alpha);
-            const float a1 = __fmul_rn(__uint_as_float(v[k8 * 8 + 2 * j + 1]), a.alpha);
-            u[j] = pack_bf16x2(a0, a1);
-          }
-          if (p.bias != nullptr) {
-            const uint4 bv = __ldg(reinterpret_cast<const uint4*>(p.bias + nf));
-            const uint32_t bw[4] = {bv.x, bv.y, bv.z, bv.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              u[j] = pack_bf16x2(__fadd_rn(lo_bf16(u[j]), lo_bf16(bw[j])), __fadd_rn(hi_bf16(u[j]), hi_bf16(bw[j])));
-          }
-          if (p.epi == LTXQ_EPI_GELU) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) u[j] = gemm::gelu_tab_x2(u[j], gtab);
-          }
-          if (m < p.M) gemm::epi_row_store(p, u, m, nf, zero8, gated, two_round, false);
-        }
+        gemm::epi_row32(p, a.alpha, v, m, n0 + c * 32, gated, two_round, gtab);
       }
       tc_fence_before();
       gemm::named_bar_sync(1, 32 * P::kEpiWarps);

@@ -31,6 +31,14 @@ struct Params {
   float alpha;  // nvfp4: the tensor scale that multiplies the accumulator (1 elsewhere)
 };
 
+// output tiles of a pair kernel, how many stay whole, K splits of the rest
+struct Sched {
+  int tiles, dp, splits;
+};
+Sched plan_schedule(int64_t M, int64_t N, int64_t K);
+size_t splitk_bytes(int64_t M, int64_t N, int64_t K);
+ltxq_status launch_splitk_reduce(const Params& p, cudaStream_t stream);
+
 // gelu_approx with the reference's per-op bf16 rounding (feed_forward.py:8-14;
 // MLX evaluates each op of the expression on bf16 arrays, the constants
 // 0.044715 and sqrt(2/pi) taking the bf16 values below).
@@ -118,6 +126,36 @@ __device__ __forceinline__ void epi_row_store(const Params& p, uint32_t (&u)[4],
     }
   }
   *reinterpret_cast<uint4*>(p.out + off) = make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+// Epilogue of 32 consecutive features [n0, n0 + 32) of token m, the fp32
+// accumulators in v (tokens on the TMEM lanes: a thread has a row): alpha, the
+// first rounding point, bias, GELU and the gated residual, 16-byte stores.
+__device__ __forceinline__ void epi_row32(const Params& p, float alpha, const uint32_t (&v)[32], int m, int n0, bool gated,
+                                          bool two_round, const uint16_t* gtab) {
+  const float zero8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k8 = 0; k8 < 4; ++k8) {
+    const int nf = n0 + k8 * 8;
+    if (nf >= p.N) break;  // uniform
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      u[j] = pack_bf16x2(__fmul_rn(__uint_as_float(v[k8 * 8 + 2 * j]), alpha),
+                         __fmul_rn(__uint_as_float(v[k8 * 8 + 2 * j + 1]), alpha));
+    if (p.bias != nullptr) {
+      const uint4 bv = __ldg(reinterpret_cast<const uint4*>(p.bias + nf));
+      const uint32_t bw[4] = {bv.x, bv.y, bv.z, bv.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        u[j] = pack_bf16x2(__fadd_rn(lo_bf16(u[j]), lo_bf16(bw[j])), __fadd_rn(hi_bf16(u[j]), hi_bf16(bw[j])));
+    }
+    if (p.epi == LTXQ_EPI_GELU) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = gelu_tab_x2(u[j], gtab);
+    }
+    if (m < p.M) epi_row_store(p, u, m, nf, zero8, gated, two_round, false);
+  }
 }
 
 // Epilogue state of one thread for a fixed chunk of 8 features [nf, nf + 8):

@@ -47,6 +47,9 @@ ltxq_status launch_qlinear_mx(const void* x, int64_t M, const ltxq_qweight& w, c
                               cudaStream_t stream);
 size_t fp4_workspace_bytes(int64_t M, const ltxq_qweight& w);
 bool fp4_rows_supported(int64_t M, const ltxq_qweight& w);
+size_t fp4_dense_bytes(int64_t M, const ltxq_qweight& w, size_t* partial_offset);
+ltxq_status launch_qlinear_fp4_dense(const void* x, const ltxq_qweight& w, gemm::Params p, void* workspace,
+                                     cudaStream_t stream);
 ltxq_status launch_fp4_rows(const void* x, bool quantize, const ltxq_fp4_act* packed, const ltxq_qweight& w,
                             const gemm::Params& p, cudaStream_t stream);
 ltxq_status launch_qlinear_fp4_from_bf16(const void* x, int64_t M, const ltxq_qweight& w, const gemm::Params& p,
@@ -72,11 +75,6 @@ constexpr int group_log2(int qk) { return qk == kNvfp4 ? 4 : 5; }
 template <int QK>
 struct QTraits {
   static constexpr int kWBytes = QK == kAffine4 || is_fp4(QK) ? 32 : 64;  // packed bytes per row per stage
-};
-
-// output tiles of the pair kernel, how many stay whole, K splits of the rest
-struct Sched {
-  int tiles, dp, splits;
 };
 
 // 16-byte blocks of a row's group parameters (8 bf16 scales / biases for
@@ -1450,6 +1448,16 @@ size_t splitk_bytes(int64_t M, int64_t N, int64_t K) {
   return sc.splits > 1 ? static_cast<size_t>(sc.tiles - sc.dp) * sc.splits * kPairTile * kPairTile * 4 : 0;
 }
 
+// the reduction of a pair schedule's split tiles (p.partial, p.dp_tiles, p.splits)
+ltxq_status launch_splitk_reduce(const Params& p, cudaStream_t stream) {
+  const int tiles = ((p.N + 2 * BM - 1) / (2 * BM)) * ((p.M + 255) / 256);
+  const int64_t items = static_cast<int64_t>(tiles - p.dp_tiles) * kPairTile * (kPairTile / 8);
+  const int64_t want = (items + 255) / 256;
+  const int cap = num_sms() * 8;
+  splitk_reduce_kernel<<<static_cast<unsigned>(want < cap ? want : cap), 256, 0, stream>>>(p);
+  return launch_check("split-K reduce launch");
+}
+
 template <int QK>
 static ltxq_status launch_qk(int bn, const CUtensorMap& tx, const CUtensorMap& tw, const Params& p,
                              cudaStream_t stream) {
@@ -1561,6 +1569,12 @@ ltxq_status launch_qlinear(const void* x, int64_t M, const ltxq_qweight& w, cons
     return launch_qlinear_fp4_from_bf16(x, M, w, p, workspace, stream);
   }
 
+  // many rows with an fp4 weight: dequantized once into the workspace
+  if (const size_t bytes = fp4_dense_bytes(M, w, nullptr)) {
+    if (workspace && workspace_bytes >= bytes && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0)
+      return launch_qlinear_fp4_dense(x, w, p, workspace, stream);
+  }
+
   // native block-scaled fp8 path (LTXQ_COMPUTE_MX*), when it applies and the
   // workspace holds the split activations
   if (const size_t mx_bytes = mx_workspace_bytes(M, w)) {
@@ -1649,6 +1663,10 @@ size_t ltxq_qlinear_workspace_size(int64_t M, const ltxq_qweight* w) {
   const size_t mx = ltxq::mx_workspace_bytes(M, *w);
   if (mx) return ltxq::align_up(mx);  // the native path runs unsplit
   if (const size_t f4 = ltxq::fp4_workspace_bytes(M, *w)) return ltxq::align_up(f4);
+  if (w->mode == LTXQ_MXFP4 || w->mode == LTXQ_NVFP4) {
+    if (ltxq::fp4_rows_supported(M, *w)) return 0;
+    if (const size_t d = ltxq::fp4_dense_bytes(M, *w, nullptr)) return ltxq::align_up(d);
+  }
   return ltxq::align_up(ltxq::gemm::splitk_bytes(M, w->n_out, w->k_in));
 }
 

@@ -9,23 +9,26 @@
 //
 // The reference keeps cos / sin tables (model/transformer/rope.py:53-90 split,
 // and its interleaved form); here the angle is formed in the kernel, so a
-// call reads x, one position per token and axis, and the frequencies.  The
-// product and its reduction to [-1/8, 1/8] of a turn are done in fp64, so that
-// positions in the millions keep the fp32 angle's last bit; cos and sin are
-// their Taylor series on that interval.
+// call reads x, one position per token and axis, and the frequencies.  Turns
+// position * frequency / (2 pi) are formed from two fp32 parts of each (48 bits,
+// the product's rounding kept by an fma) and reduced to [-1/8, 1/8] exactly: the
+// error is turns * 2^-47, below the fp32 angle's last bit up to 2^20 turns (6.6
+// million radians); beyond, the product is taken in fp64.  cos and sin are their
+// Taylor series on the interval, or for bf16 the hardware's functions.
 //
-// Memory-bound: 2 reads/writes of x.  A thread keeps V neighbouring pairs of
-// one head (two 16-byte loads) and walks tokens, so its frequencies stay in
-// registers.  Where all heads share the frequencies the angles of a CTA's
-// tokens are computed once into shared memory; with a row of frequencies per
-// head every pair has its own angle and each thread computes its own.
+// Memory-bound where the heads share the frequencies: the angles of a CTA's
+// rows are computed once into shared memory, and its threads walk (row, unit)
+// items, a unit being V neighbouring pairs of one head, two vectors of 16 bytes.
+// With a row of frequencies per head every pair has its own angle (about 40
+// instructions); a thread keeps one unit's frequencies in registers and walks
+// rows, loading the next one's x ahead.
 #include "common.cuh"
 
 namespace ltxq {
 namespace rotary {
 
 constexpr int kThreads = 256;
-constexpr int kTableMax = 2048;  // (cos, sin) pairs of one CTA's tokens, 16 KB
+constexpr int kTableMax = 2048;  // (cos, sin) pairs of one CTA's rows, or its (high, low) positions: 16 KB
 
 struct Args {
   const void* x;
@@ -38,10 +41,10 @@ struct Args {
   int64_t rows;  // batch * tokens
   int tokens, heads, d, half;
   int n_axes, pos_type, per_head;
-  int units;      // per row: heads * (rotated units + copied units)
+  int units;      // per row: heads * (rotated units + units that pass through)
   int rot_units;  // per head
   int all_units;  // per head
-  int rows_per_cta;
+  int rows_per_cta, units_per_cta;
   float scale;
   int inverse;
 };
@@ -56,14 +59,9 @@ __device__ __forceinline__ double load_pos(const Args& a, int64_t b, int64_t t, 
   }
 }
 
-// cos and sin of 2 pi t.  t = q / 4 + r with an integer q and |r| <= 1/8: the
-// reduction is exact in fp64, r then fits fp32 to 2^-28 of a turn.
-__device__ __forceinline__ void cos_sin_turns(double t, float& c, float& s) {
-  if (!(fabs(t) < 1e15)) t = t - rint(t);  // keeps 4t inside the adding trick's range; NaN and infinity give NaN
-  constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
-  const double m = __dadd_rn(4.0 * t, kRound);
-  const int q = __double2loint(m);
-  const float z = static_cast<float>(__fma_rn(__dsub_rn(m, kRound), -0.25, t)) * 6.283185307179586f;
+// cos and sin of q / 4 + r turns, |r| <= 1/8
+__device__ __forceinline__ void cos_sin_part(int q, float r, float& c, float& s) {
+  const float z = r * 6.283185307179586f;
   const float z2 = z * z;
   // |z| <= pi/4: the first terms left out are below 2e-9 (sin) and 2e-10 (cos)
   float sn = fmaf(z2, 2.7557319224e-6f, -1.9841269841e-4f);
@@ -76,134 +74,280 @@ __device__ __forceinline__ void cos_sin_turns(double t, float& c, float& s) {
   cs = fmaf(z2, cs, -0.5f);
   cs = fmaf(z2, cs, 1.0f);
   const bool swap = q & 1;
-  c = swap ? sn : cs;
-  s = swap ? cs : sn;
-  if ((q + 1) & 2) c = -c;  // quadrants 1, 2
-  if (q & 2) s = -s;        // quadrants 2, 3
+  // cos is negative in quadrants 1 and 2, sin in 2 and 3
+  c = __uint_as_float(__float_as_uint(swap ? sn : cs) ^ ((static_cast<uint32_t>(q + 1) << 30) & 0x80000000u));
+  s = __uint_as_float(__float_as_uint(swap ? cs : sn) ^ ((static_cast<uint32_t>(q) << 30) & 0x80000000u));
+}
+
+// cos and sin of t turns, any t: t = q / 4 + r, exact in fp64
+__device__ __noinline__ void cos_sin_far(double t, float& c, float& s) {
+  if (!(fabs(t) < 1e15)) t = t - rint(t);  // keeps 4t inside the adding trick's range; NaN and infinity give NaN
+  constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
+  const double m = __dadd_rn(4.0 * t, kRound);
+  cos_sin_part(__double2loint(m), static_cast<float>(__fma_rn(__dsub_rn(m, kRound), -0.25, t)), c, s);
 }
 
 constexpr double kInvTwoPi = 0.15915494309189535;
 
-__device__ __forceinline__ float2 angle(const Args& a, double turns) {
-  float c, s;
-  cos_sin_turns(turns, c, s);
-  return make_float2(c * a.scale, (a.inverse ? -s : s) * a.scale);
+// an fp64 value as the sum of two fp32 ones
+__device__ __forceinline__ float2 split2(double v) {
+  const float hi = static_cast<float>(v);
+  return make_float2(hi, static_cast<float>(v - static_cast<double>(hi)));
 }
 
+constexpr float kFarTurns = 1048576.0f;
+
+// cos and sin of p * f turns, both as two parts, |p * f| < kFarTurns.  kShort:
+// for results that are rounded to bf16, the hardware's functions (off by at most
+// 2^-20.9 within a turn, where bf16 rounds by 2^-9 of a value): with them the
+// video grid's case is bound by memory, with the series by instructions.
+template <bool kShort>
+__device__ __forceinline__ void cos_sin(float2 p, float2 f, float& c, float& s) {
+  const float t = __fmul_rn(p.x, f.x);
+  const float e = fmaf(p.x, f.x, -t) + fmaf(p.x, f.y, p.y * f.x);
+  constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer
+  if (kShort) {
+    const float m = t + kRound;
+    const float z = ((t - (m - kRound)) + e) * 6.283185307179586f;
+    c = __cosf(z);
+    s = __sinf(z);
+  } else {
+    const float m = fmaf(t, 4.0f, kRound);
+    cos_sin_part(__float_as_int(m), fmaf(m - kRound, -0.25f, t) + e, c, s);
+  }
+}
+
+// V elements as they lie in memory, and as fp32
 template <typename T, int V>
-struct Vec {
-  float v[V];
+struct Raw {
+  static constexpr int kBytes = sizeof(T) * V;
+  uint32_t w[(kBytes + 3) / 4];
   __device__ __forceinline__ void load(const T* p) {
-    if constexpr (sizeof(T) * V == 16) {
-      const uint4 w = *reinterpret_cast<const uint4*>(p);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 2) {
-          v[2 * i] = lo_bf16(u[i]);
-          v[2 * i + 1] = hi_bf16(u[i]);
-        } else {
-          v[i] = __uint_as_float(u[i]);
-        }
-      }
+    if constexpr (kBytes == 16) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else if constexpr (kBytes == 8) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      w[0] = u.x; w[1] = u.y;
+    } else if constexpr (kBytes == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
     } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = sizeof(T) == 2 ? bf16_to_f32(reinterpret_cast<const uint16_t*>(p)[i])
-                                                        : reinterpret_cast<const float*>(p)[i];
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
     }
   }
   __device__ __forceinline__ void store(T* p) const {
-    if constexpr (sizeof(T) * V == 16) {
-      uint32_t u[4];
+    if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else if constexpr (kBytes == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+    else *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[0]);
+  }
+  __device__ __forceinline__ void get(float (&v)[V]) const {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = sizeof(T) == 2 ? pack_bf16x2(v[2 * i % V], v[(2 * i + 1) % V]) : __float_as_uint(v[i]);
-      *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
-    } else {
+    for (int i = 0; i < V; ++i) {
+      if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
+      else v[i] = i & 1 ? hi_bf16(w[i / 2]) : lo_bf16(w[i / 2]);
+    }
+  }
+  __device__ __forceinline__ void put(const float (&v)[V]) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if constexpr (sizeof(T) == 2) reinterpret_cast<uint16_t*>(p)[i] = f32_to_bf16(v[i]);
-        else reinterpret_cast<float*>(p)[i] = v[i];
-      }
+    for (int i = 0; i < V; ++i) {
+      if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+      else if constexpr (V == 1) w[0] = f32_to_bf16(v[0]);
+      else if (i % 2 == 0) w[i / 2] = pack_bf16x2(v[i], v[(i + 1) % V]);
     }
   }
 };
 
-// T: uint16_t (bf16) or float.  V pairs per unit: 16 bytes of each of the two
-// vectors, or 1 where alignment or sizes leave no wider form.
-template <typename T, int V, bool kHalf, bool kPerHead>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const Args a) {
-  __shared__ float2 table[kPerHead ? 1 : kTableMax];
+// Where a unit's two vectors lie in its head: pairs of both halves, neighbours
+// of the interleaved layout, or elements that pass through.
+template <int V, bool kHalf>
+struct Unit {
+  int e0, e1;
+  bool rot, second;
+  __device__ __forceinline__ Unit(const Args& a, int c) {
+    rot = c < a.rot_units;
+    e0 = !rot ? 2 * a.half + (c - a.rot_units) * 2 * V : kHalf ? c * V : c * 2 * V;
+    e1 = rot && kHalf ? e0 + a.half : e0 + V;
+    second = rot || e1 < a.d;  // an odd head: the last unit that passes through is one element
+  }
+};
+
+// rotates the V pairs of p, q; cs[i]: (cos, sin) of pair i
+template <typename T, int V, bool kHalf>
+__device__ __forceinline__ void rotate(Raw<T, V>& p, Raw<T, V>& q, const float2 (&cs)[V]) {
+  float x[V], y[V];
+  p.get(x);
+  q.get(y);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    // interleaved: pair i is elements 2i, 2i + 1 of the unit's 2V
+    float& m = kHalf ? x[i] : (2 * i < V ? x[2 * i % V] : y[2 * i % V]);
+    float& o = kHalf ? y[i] : (2 * i + 1 < V ? x[(2 * i + 1) % V] : y[(2 * i + 1) % V]);
+    const float mu = m, mv = o;
+    m = fmaf(mu, cs[i].x, -(mv * cs[i].y));
+    o = fmaf(mv, cs[i].x, mu * cs[i].y);
+  }
+  p.put(x);
+  q.put(y);
+}
+
+// Heads that share the frequencies.  T: uint16_t (bf16) or float.  V pairs per
+// unit: 16 bytes of each vector, or less where alignment or sizes leave no
+// wider form.
+template <typename T, int V, bool kHalf>
+__global__ void __launch_bounds__(kThreads) rotary_shared_kernel(const Args a) {
+  __shared__ float2 table[kTableMax];
   const int64_t row0 = blockIdx.x * static_cast<int64_t>(a.rows_per_cta);
   const int n = static_cast<int>(min(static_cast<int64_t>(a.rows_per_cta), a.rows - row0));
-  if (!kPerHead) {
-    for (int i = threadIdx.x; i < n * a.half; i += kThreads) {
-      const int r = i / a.half, k = i - r * a.half;
-      const int64_t row = row0 + r;
-      const int64_t b = row / a.tokens, t = row - b * a.tokens;
-      const int ax = a.axis ? __ldg(a.axis + k) : 0;
-      const double p = static_cast<unsigned>(ax) < static_cast<unsigned>(a.n_axes) ? load_pos(a, b, t, ax) : NAN;
-      table[i] = angle(a, p * (__ldg(a.freqs + k) * kInvTwoPi));
+  // this CTA's share of the rows' units; an item's x is loaded one item ahead, the first one's before the table
+  const int u0 = blockIdx.y * a.units_per_cta, nu = min(a.units_per_cta, a.units - u0);
+  const int dr = kThreads / nu, du = kThreads - dr * nu;
+  int nr = threadIdx.x / nu, ru = threadIdx.x - nr * nu;  // the item loaded next
+  Raw<T, V> p, q;
+  T* out = nullptr;
+  int c = 0, r = nr;
+  auto load = [&] {
+    const int h = (u0 + ru) / a.all_units;
+    c = u0 + ru - h * a.all_units;
+    r = nr;
+    const Unit<V, kHalf> w(a, c);
+    const int64_t row = row0 + nr;
+    const int64_t b = row / a.tokens, t = row - b * a.tokens;
+    const T* x = static_cast<const T*>(a.x) + b * a.xs[0] + t * a.xs[1] + h * a.xs[2];
+    out = static_cast<T*>(a.out) + b * a.os[0] + t * a.os[1] + h * a.os[2];
+    p.load(x + w.e0);
+    if (w.second) q.load(x + w.e1);
+    nr += dr;
+    ru += du;
+    if (ru >= nu) {
+      ru -= nu;
+      ++nr;
     }
-    __syncthreads();
+  };
+  if (nr < n) load();
+  for (int i = threadIdx.x; i < n * a.half; i += kThreads) {
+    const int tr = i / a.half, k = i - tr * a.half;
+    const int64_t row = row0 + tr;
+    const int64_t b = row / a.tokens, t = row - b * a.tokens;
+    const int ax = a.axis ? __ldg(a.axis + k) : 0;
+    const double v = static_cast<unsigned>(ax) < static_cast<unsigned>(a.n_axes) ? load_pos(a, b, t, ax) : NAN;
+    const double f = __ldg(a.freqs + k) * kInvTwoPi;
+    const float2 ph = split2(a.inverse ? -v : v), fh = split2(f);
+    float co, si;
+    if (fabsf(ph.x * fh.x) < kFarTurns) cos_sin<sizeof(T) == 2>(ph, fh, co, si);
+    else cos_sin_far(a.inverse ? -v * f : v * f, co, si);
+    table[i] = make_float2(co * a.scale, si * a.scale);
   }
+  __syncthreads();
+  while (r < n) {
+    Raw<T, V> m = p, o = q;
+    T* const at = out;
+    const int mc = c, mr = r;
+    if (nr < n) load();
+    else r = n;
+    const Unit<V, kHalf> w(a, mc);
+    if (w.rot) {
+      float2 cs[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) cs[i] = table[mr * a.half + mc * V + i];
+      rotate<T, V, kHalf>(m, o, cs);
+    }
+    m.store(at + w.e0);
+    if (w.second) o.store(at + w.e1);
+  }
+}
+
+// A row of frequencies for each head.
+template <typename T, int V, bool kHalf>
+__global__ void __launch_bounds__(kThreads) rotary_heads_kernel(const Args a) {
+  __shared__ float2 pos[kTableMax];  // [row][axis]
+  const int64_t row0 = blockIdx.x * static_cast<int64_t>(a.rows_per_cta);
+  const int n = static_cast<int>(min(static_cast<int64_t>(a.rows_per_cta), a.rows - row0));
+  for (int i = threadIdx.x; i < n * a.n_axes; i += kThreads) {
+    const int r = i / a.n_axes, ax = i - r * a.n_axes;
+    const int64_t row = row0 + r;
+    const int64_t b = row / a.tokens, t = row - b * a.tokens;
+    const double p = load_pos(a, b, t, ax);
+    pos[i] = split2(a.inverse ? -p : p);
+  }
+  __syncthreads();
   const int u = blockIdx.y * kThreads + threadIdx.x;
   if (u >= a.units) return;
   const int h = u / a.all_units, c = u - h * a.all_units;
-  const bool rot = c < a.rot_units;
-  // first element of the unit's two vectors within the head
-  const int e0 = !rot ? 2 * a.half + (c - a.rot_units) * 2 * V : kHalf ? c * V : c * 2 * V;
-  const int e1 = rot && kHalf ? e0 + a.half : e0 + V;
-  const bool second = rot || e1 < a.d;  // an odd head: the last copied unit is one element
-  double f[kPerHead ? V : 1];
-  int ax[kPerHead ? V : 1];
-  if (kPerHead && rot) {
+  const Unit<V, kHalf> w(a, c);
+  float2 f[V];
+  int ax[V];
+  if (w.rot) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      f[i] = __ldg(a.freqs + h * a.half + c * V + i) * kInvTwoPi;
-      ax[i] = a.axis ? __ldg(a.axis + h * a.half + c * V + i) : 0;
+      const int k = h * a.half + c * V + i;
+      f[i] = split2(__ldg(a.freqs + k) * kInvTwoPi);
+      ax[i] = a.axis ? __ldg(a.axis + k) : 0;
       if (static_cast<unsigned>(ax[i]) >= static_cast<unsigned>(a.n_axes)) {
-        f[i] = NAN;
+        f[i].x = NAN;
         ax[i] = 0;
       }
     }
   }
   const T* x = static_cast<const T*>(a.x) + h * a.xs[2];
   T* out = static_cast<T*>(a.out) + h * a.os[2];
-  for (int r = 0; r < n; ++r) {
-    const int64_t row = row0 + r;
-    const int64_t b = row / a.tokens, t = row - b * a.tokens;
+  int64_t b = row0 / a.tokens, t = row0 - b * a.tokens;
+  Raw<T, V> p, q;
+  auto load = [&] {
     const T* xr = x + b * a.xs[0] + t * a.xs[1];
+    p.load(xr + w.e0);
+    if (w.second) q.load(xr + w.e1);
+  };
+  load();
+#pragma unroll 1
+  for (int r = 0; r < n; ++r) {
     T* orow = out + b * a.os[0] + t * a.os[1];
-    Vec<T, V> p, q;
-    p.load(xr + e0);
-    if (second) q.load(xr + e1);
-    if (rot) {
+    const int64_t b0 = b, t0 = t;
+    Raw<T, V> m = p, o = q;
+    if (++t == a.tokens) {
+      t = 0;
+      ++b;
+    }
+    if (r + 1 < n) load();
+    if (w.rot) {
+      float2 ph[V], cs[V];
+      float most = 0.f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        float2 cs;
-        if (kPerHead) cs = angle(a, load_pos(a, b, t, ax[kPerHead ? i : 0]) * f[kPerHead ? i : 0]);
-        else cs = table[r * a.half + c * V + i];
-        // interleaved: pair i is elements 2i, 2i + 1 of the unit's 2V
-        float& m = kHalf ? p.v[i] : (2 * i < V ? p.v[2 * i % V] : q.v[2 * i % V]);
-        float& o = kHalf ? q.v[i] : (2 * i + 1 < V ? p.v[(2 * i + 1) % V] : q.v[(2 * i + 1) % V]);
-        const float mu = m, mv = o;
-        m = fmaf(mu, cs.x, -(mv * cs.y));
-        o = fmaf(mv, cs.x, mu * cs.y);
+        ph[i] = pos[r * a.n_axes + ax[i]];
+        most = fmaxf(most, fabsf(ph[i].x * f[i].x));
       }
+      if (most < kFarTurns) {  // NaN falls out of fmaxf and is NaN below too
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float c1, s1;
+          cos_sin<sizeof(T) == 2>(ph[i], f[i], c1, s1);
+          cs[i] = make_float2(c1 * a.scale, s1 * a.scale);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const double v = load_pos(a, b0, t0, ax[i]) * (__ldg(a.freqs + h * a.half + c * V + i) * kInvTwoPi);
+          float c1, s1;
+          cos_sin_far(isnan(f[i].x) ? static_cast<double>(NAN) : a.inverse ? -v : v, c1, s1);
+          cs[i] = make_float2(c1 * a.scale, s1 * a.scale);
+        }
+      }
+      rotate<T, V, kHalf>(m, o, cs);
     }
-    p.store(orow + e0);
-    if (second) q.store(orow + e1);
+    m.store(orow + w.e0);
+    if (w.second) o.store(orow + w.e1);
   }
 }
 
 template <typename T, int V>
 static void launch(const Args& a, bool half_layout, dim3 grid, cudaStream_t s) {
   if (half_layout) {
-    if (a.per_head) rotary_kernel<T, V, true, true><<<grid, kThreads, 0, s>>>(a);
-    else rotary_kernel<T, V, true, false><<<grid, kThreads, 0, s>>>(a);
+    if (a.per_head) rotary_heads_kernel<T, V, true><<<grid, kThreads, 0, s>>>(a);
+    else rotary_shared_kernel<T, V, true><<<grid, kThreads, 0, s>>>(a);
   } else {
-    if (a.per_head) rotary_kernel<T, V, false, true><<<grid, kThreads, 0, s>>>(a);
-    else rotary_kernel<T, V, false, false><<<grid, kThreads, 0, s>>>(a);
+    if (a.per_head) rotary_heads_kernel<T, V, false><<<grid, kThreads, 0, s>>>(a);
+    else rotary_shared_kernel<T, V, false><<<grid, kThreads, 0, s>>>(a);
   }
 }
 
@@ -241,17 +385,19 @@ extern "C" ltxq_status ltxq_rotary(const ltxq_rotary_args* r, void* stream) {
   a.x = r->x;
   a.out = r->out;
   const int64_t half = r->rotary_dim / 2;
-  const int wide = 16 / es;
-  // 16-byte vectors: both vectors of every unit start on 16 bytes
-  bool vec = half % wide == 0 && r->head_dim % (2 * wide) == 0 &&
-             ((reinterpret_cast<uintptr_t>(r->x) | reinterpret_cast<uintptr_t>(r->out)) & 15u) == 0;
+  // V: the widest vectors that start on their own size, 16 bytes, two elements or one
+  auto fits = [&](int v) {
+    bool ok = half % v == 0 && r->head_dim % (2 * v) == 0 &&
+              ((reinterpret_cast<uintptr_t>(r->x) | reinterpret_cast<uintptr_t>(r->out)) % (v * es)) == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && r->x_stride[i] % v == 0 && r->out_stride[i] % v == 0;
+    return ok;
+  };
+  const int V = fits(16 / es) ? 16 / es : fits(2) ? 2 : 1;
   for (int i = 0; i < 3; ++i) {
     a.xs[i] = r->x_stride[i];
     a.os[i] = r->out_stride[i];
     a.ps[i] = r->pos_stride[i];
-    vec = vec && a.xs[i] % wide == 0 && a.os[i] % wide == 0;
   }
-  const int V = vec ? wide : 1;
   a.pos = r->positions;
   a.freqs = r->freqs;
   a.axis = r->axis;
@@ -268,11 +414,26 @@ extern "C" ltxq_status ltxq_rotary(const ltxq_rotary_args* r, void* stream) {
   a.units = a.heads * a.all_units;
   a.scale = r->scale;
   a.inverse = r->inverse ? 1 : 0;
-  // rows per CTA: as many as leave every SM several CTAs, within the shared table
-  const int64_t gy = (a.units + kThreads - 1) / kThreads;
-  int64_t per = a.rows * gy / (static_cast<int64_t>(num_sms()) * 8);
-  if (!a.per_head && a.half > 0 && per > kTableMax / a.half) per = kTableMax / a.half;
-  per = per < 1 ? 1 : (per > 16 ? 16 : per);
+  if (a.per_head && a.n_axes > kTableMax) return fail(LTXQ_ERR_UNSUPPORTED, "rotary: at most 2048 position axes");
+  // Rows per CTA, within the table: shared frequencies, 1024 items of work (a few per thread, the table's cost spread
+  // over every head); a row of frequencies per head, 16 rows for a thread's registers.  Fewer where that would leave
+  // SMs idle.
+  int64_t per, gy;
+  const int sms = num_sms();
+  if (a.per_head) {
+    gy = (a.units + kThreads - 1) / kThreads;
+    per = 16;
+    if (per > kTableMax / a.n_axes) per = kTableMax / a.n_axes;
+    a.units_per_cta = kThreads;
+  } else {
+    a.units_per_cta = a.units < 1024 ? a.units : 1024;
+    gy = (a.units + a.units_per_cta - 1) / a.units_per_cta;
+    per = 1024 / a.units_per_cta;
+    if (a.half > 0 && per > kTableMax / a.half) per = kTableMax / a.half;
+  }
+  const int64_t enough = (a.rows * gy + 4 * sms - 1) / (4 * sms);
+  if (per > enough) per = enough;
+  if (per < 1) per = 1;
   const int64_t gx = (a.rows + per - 1) / per;
   if (gy > 65535 || gx > 0x7FFFFFFF) return fail(LTXQ_ERR_UNSUPPORTED, "rotary: dimension too large");
   a.rows_per_cta = static_cast<int>(per);
@@ -280,10 +441,12 @@ extern "C" ltxq_status ltxq_rotary(const ltxq_rotary_args* r, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool hl = r->layout == LTXQ_ROTARY_HALF;
   if (es == 2) {
-    if (vec) launch<uint16_t, 8>(a, hl, grid, s);
+    if (V == 8) launch<uint16_t, 8>(a, hl, grid, s);
+    else if (V == 2) launch<uint16_t, 2>(a, hl, grid, s);
     else launch<uint16_t, 1>(a, hl, grid, s);
   } else {
-    if (vec) launch<float, 4>(a, hl, grid, s);
+    if (V == 4) launch<float, 4>(a, hl, grid, s);
+    else if (V == 2) launch<float, 2>(a, hl, grid, s);
     else launch<float, 1>(a, hl, grid, s);
   }
   return launch_check("rotary launch");

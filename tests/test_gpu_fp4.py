@@ -180,7 +180,7 @@ def test_quantize_strided_empty_and_refused(cuda):
 
 PRODUCTS = [(1, 8, 32), (1, 16, 64), (2, 24, 96), (5, 136, 288), (8, 1024, 512), (9, 1048, 2080), (17, 200, 1056),
             (64, 256, 256), (65, 264, 320), (129, 384, 2048), (200, 2048, 1024), (257, 520, 4096), (513, 192, 544),
-            (700, 4096, 256), (2050, 4104, 800)]
+            (700, 4096, 256), (1030, 264, 96), (1200, 2056, 544), (2050, 4104, 800)]
 
 
 @pytest.mark.parametrize("mode", MODES)
