@@ -184,13 +184,11 @@ ltxq_status launch_fp4_dequantize_rows(const uint8_t* codes, const uint8_t* scal
 namespace fp4 {
 
 // Persistent kernel, clusters of two CTAs (tcgen05 cta_group::2).  A tile is
-// 256 kBlocks tokens x 192 features: CTA r holds kBlocks blocks of 128 token
-// rows (operand A, TMEM lanes = tokens) and 96 weight rows (operand B).  Codes
+// 256 kBlocks tokens x BN features: CTA r holds kBlocks blocks of 128 token
+// rows (operand A, TMEM lanes = tokens) and BN / 2 weight rows (operand B).  Codes
 // of a 256-K stage (128-byte swizzle) arrive by TMA on one barrier of the
-// leader, scale atoms on one of each CTA's own.  With tokens on the lanes an
-// epilogue thread holds 32 consecutive features of one row: bias, GELU and the
-// gated residual need no transpose, and 64 contiguous bytes of each row are
-// written.
+// leader, scale atoms on one of each CTA's own.  With tokens on the lanes
+// an epilogue thread holds consecutive features of one row.
 //
 // The MMA reads its scales from tensor memory: of rows m and 32 + m, 64 + m,
 // 96 + m on lane m, the same in all four lane quarters.  Four warps per CTA,
@@ -200,22 +198,22 @@ namespace fp4 {
 // own time, 54 cycles an atom: at 9216 x 16384 x 4096 nvfp4 the MMAs alone took
 // 213 us, the copies alone 190 more, and the kernel 414.
 constexpr int BM = 128;       // tokens per block and CTA (MMA M = 256 for the pair)
-constexpr int BN = 192;       // features per tile (MMA N)
-constexpr int BNC = BN / 2;   // weight rows per CTA
 constexpr int BKB = kStageK / 2;  // bytes of one operand row in a stage
 constexpr uint32_t kTmemCols = 512;
 constexpr int kGroupM = 16;  // token tiles that walk the feature tiles together (L2 reuse of the weight)
 
-template <int F, int kBlocks>
+template <int F, int kBlocks, int BN>
 struct Plan {
+  static constexpr int BNC = BN / 2;  // weight rows per CTA
   static constexpr int AP = Traits<F>::kAtoms;
   static constexpr int kA = kBlocks * BM * BKB;       // this CTA's token rows
   static constexpr int kB = BNC * BKB;                // this CTA's weight rows
   static constexpr int kSfa = kBlocks * AP * kAtom;   // its tokens' scales
-  static constexpr int kSfb = 2 * AP * kAtom;         // the two 128-feature row tiles that 192 features touch
+  static constexpr int kSfb = 2 * AP * kAtom;         // the two 128-feature row tiles that BN features touch
   static constexpr int kStage = kA + kB + kSfa + kSfb;
   static constexpr uint32_t kStageTx = 2u * (kA + kB);  // both CTAs' codes land on the leader's barrier
-  static constexpr int kEpiWarps = 4 * kBlocks;
+  static constexpr int kEpiWarps = 8;  // per lane quarter: one for each block, or two for the columns of one
+  static constexpr int kParts = 2 / kBlocks;
   static constexpr int kSfWarp0 = kEpiWarps;  // four warps that bring scales to TMEM
   static constexpr int kTmaWarp = kEpiWarps + 4, kMmaWarp = kEpiWarps + 5;
   static constexpr int kThreads = 32 * (kEpiWarps + 6);
@@ -234,6 +232,8 @@ struct Plan {
   static constexpr uint32_t kSfbOffCol = 4 * kBlocks * AP;
   static constexpr uint32_t kSfCols = (kSfbOffCol + 8 * AP + 15) / 16 * 16;  // stores are 16 columns wide
   static_assert(kSfCol + 2 * kSfCols <= kTmemCols, "TMEM columns");
+  // a tile starts 0 or 64 features into a row tile, 0 or 2 columns into its scales: the MMA faults on odd columns
+  static_assert(BN % 64 == 0 && BN <= 192, "tile width");
   static_assert(kStages >= 4, "pipeline depth");
   static_assert(kSmem <= 227 * 1024, "shared memory budget");
   static_assert(kA % 1024 == 0 && kB % 1024 == 0, "128B-swizzle atoms need 1024-byte alignment");
@@ -273,12 +273,12 @@ struct GemmArgs {
   float alpha;           // product of the operands' global scales
 };
 
-template <int F, int kBlocks>
-__global__ void __launch_bounds__(Plan<F, kBlocks>::kThreads, 1)
+template <int F, int kBlocks, int BN>
+__global__ void __launch_bounds__(Plan<F, kBlocks, BN>::kThreads, 1)
     qgemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_sfx,
                           const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_sfw,
                           const GemmArgs a, const gemm::Params p) {
-  using P = Plan<F, kBlocks>;
+  using P = Plan<F, kBlocks, BN>;
   constexpr int S = P::kStages;
   constexpr int AP = P::AP;
   constexpr int kRows = kBlocks * BM;  // token rows per CTA
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(Plan<F, kBlocks>::kThreads, 1)
           if (leader) mbar_arrive_expect_tx(&full[s], P::kStageTx);
           const uint32_t bar = leader_full + 8u * s;
           tma_load_2d_pair(smem + s * P::kA, &tmap_x, bar, kb * BKB, m0);
-          tma_load_2d_pair(smem + P::kBOff + s * P::kB, &tmap_w, bar, kb * BKB, n0 + static_cast<int>(rank) * BNC);
+          tma_load_2d_pair(smem + P::kBOff + s * P::kB, &tmap_w, bar, kb * BKB, n0 + static_cast<int>(rank) * P::BNC);
           mbar_arrive_expect_tx(&sf_full[s], P::kSfa + P::kSfb);
           tma_load_2d(smem + P::kSfaOff + s * P::kSfa, &tmap_sfx, &sf_full[s], 0, (kb * a.x_tiles + m0 / BM) * AP);
           tma_load_2d(smem + P::kSfbOff + s * P::kSfb, &tmap_sfw, &sf_full[s], 0, (kb * a.w_tiles + n0 / 128) * AP);
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(Plan<F, kBlocks>::kThreads, 1)
         const int buf = it % P::kAccBufs;
         if (!mbar_wait(&acc_empty[buf], ((it / P::kAccBufs) & 1) ^ 1, abort_flag, p.err)) break;
         tc_fence_after();
-        const uint32_t skip = (n0 & 127) ? 2u : 0u;  // a tile that starts 64 features into a row tile
+        const uint32_t skip = static_cast<uint32_t>(n0 & 127) / 32;  // where the tile starts within its row tile
         for (int kb = 0; kb < num_kb; ++kb, ++g) {
           const int s = g % S;
           const int sb = g & 1;
@@ -473,7 +473,8 @@ __global__ void __launch_bounds__(Plan<F, kBlocks>::kThreads, 1)
   } else {
     // ------------------------------------------------ epilogue warps
     const int q = warp & 3;     // TMEM lane quarter of this warp
-    const int blk = warp >> 2;  // its block of token rows
+    const int blk = kBlocks == 2 ? warp >> 2 : 0;   // its block of token rows
+    const int part = kBlocks == 2 ? 0 : warp >> 2;  // its share of the columns
     const uint32_t t_lane = static_cast<uint32_t>(q * 32) << 16;
     const bool gated = p.epi == LTXQ_EPI_GATED_RESIDUAL || p.epi == LTXQ_EPI_GATE_THEN_ADD;
     const bool two_round = p.epi == LTXQ_EPI_GATE_THEN_ADD || p.gate.dtype == LTXQ_BF16;
@@ -488,14 +489,15 @@ __global__ void __launch_bounds__(Plan<F, kBlocks>::kThreads, 1)
       if (!mbar_wait(&acc_full[buf], (it / P::kAccBufs) & 1, abort_flag, p.err)) break;
       tc_fence_after();
       const uint32_t tacc = tmem + t_lane + static_cast<uint32_t>((kBlocks == 1 ? buf : blk) * BN);
-      const int m = m0 + blk * BM + q * 32 + lane;
+      const int m0w = m0 + blk * BM + q * 32;  // first token of this warp
 #pragma unroll 1
-      for (int c = 0; c < BN / 32; ++c) {
+      for (int c = part; c < BN / 32; c += P::kParts) {
         if (n0 + c * 32 >= p.N) break;  // uniform
-        uint32_t v[32];
+        uint32_t v[32], u[4][4];
         tmem_ld_32x32b_x32(tacc + c * 32, v);
         tmem_wait_ld();
-        gemm::epi_row32(p, a.alpha, v, m, n0 + c * 32, gated, two_round, gtab);
+        gemm::epi_pack32(a.alpha, v, u);
+        gemm::epi_rows32(p, u, m0w, n0 + c * 32, gated, two_round, gtab);
       }
       tc_fence_before();
       gemm::named_bar_sync(1, 32 * P::kEpiWarps);
@@ -542,16 +544,16 @@ static ltxq_status check_act(const ltxq_fp4_act* a, int64_t M, int64_t K, float*
   return fp4_global_scale(a->mode, a->global_scale, g, what);
 }
 
-template <int F, int kBlocks>
+template <int F, int kBlocks, int BN>
 static ltxq_status launch_pair(const ltxq_fp4_act& x, const ltxq_qweight& w, const GemmArgs& a, const gemm::Params& p,
                                cudaStream_t stream) {
-  using PL = Plan<F, kBlocks>;
+  using PL = Plan<F, kBlocks, BN>;
   const Sizes sx = sizes(p.M, p.K, x.mode), sw = sizes(p.N, p.K, x.mode);
   CUtensorMap tx, tsx, tw, tsw;
   if (ltxq_status st = encode_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, x.codes, p.K / 2, p.M, p.K / 2, BKB,
                                       kBlocks * BM, CU_TENSOR_MAP_SWIZZLE_128B))
     return st;
-  if (ltxq_status st = encode_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, w.weight, p.K / 2, p.N, p.K / 2, BKB, BNC,
+  if (ltxq_status st = encode_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, w.weight, p.K / 2, p.N, p.K / 2, BKB, PL::BNC,
                                       CU_TENSOR_MAP_SWIZZLE_128B))
     return st;
   // scale atoms as rows of 128 words
@@ -561,7 +563,7 @@ static ltxq_status launch_pair(const ltxq_fp4_act& x, const ltxq_qweight& w, con
   if (ltxq_status st = encode_tmap_2d(&tsw, CU_TENSOR_MAP_DATA_TYPE_UINT32, w.mx_scales, 128, sw.scales / kAtom, kAtom,
                                       128, 2 * PL::AP, CU_TENSOR_MAP_SWIZZLE_NONE))
     return st;
-  auto kern = qgemm_fp4_pair_kernel<F, kBlocks>;
+  auto kern = qgemm_fp4_pair_kernel<F, kBlocks, BN>;
   if (ltxq_status st = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PL::kSmem),
                                   "smem attribute"))
     return st;
@@ -585,13 +587,16 @@ static ltxq_status launch_pair(const ltxq_fp4_act& x, const ltxq_qweight& w, con
   return cuda_check(e, "fp4 block-scaled GEMM launch");
 }
 
+// 512 x 192 tiles where they fill every cluster once (fewest bytes per MMA: 282
+// us against 324 with 256 x 192 at 9216 x 16384 x 4096), else 256 x 192.
+// (256 x 128, 48 tiles instead of 33 at 751 x 2048 x 2048: 11.4 us, as before.)
 template <int F>
 static ltxq_status launch_gemm(const ltxq_fp4_act& x, const ltxq_qweight& w, const GemmArgs& a, const gemm::Params& p,
                                cudaStream_t stream) {
-  const int64_t n_t = (p.N + BN - 1) / BN;
+  const int64_t n_t = (p.N + 191) / 192;
   const int clusters = num_sms() / 2;
-  return (p.M + 511) / 512 * n_t >= clusters ? launch_pair<F, 2>(x, w, a, p, stream)
-                                             : launch_pair<F, 1>(x, w, a, p, stream);
+  return (p.M + 511) / 512 * n_t >= clusters ? launch_pair<F, 2, 192>(x, w, a, p, stream)
+                                             : launch_pair<F, 1, 192>(x, w, a, p, stream);
 }
 
 }  // namespace fp4

@@ -32,7 +32,7 @@ constexpr int BM = 128;  // tokens per CTA
 constexpr int BN = 256;  // features per tile
 constexpr int BK = 64;   // K per stage (128 bytes of a row)
 constexpr uint32_t kTmemCols = 512;
-constexpr int kEpiWarps = 4, kTmaWarp = 4, kMmaWarp = 5, kThreads = 192;
+constexpr int kEpiWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kThreads = 320;  // two epilogue warps per lane quarter
 constexpr int kGroupM = 16;  // token tiles that walk the feature tiles together (L2 reuse of the weight)
 
 struct Plan {
@@ -187,7 +187,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    const uint32_t t_lane = static_cast<uint32_t>(warp * 32) << 16;
+    const int q = warp & 3;  // TMEM lane quarter
+    const uint32_t t_lane = static_cast<uint32_t>(q * 32) << 16;
     const bool gated = p.epi == LTXQ_EPI_GATED_RESIDUAL || p.epi == LTXQ_EPI_GATE_THEN_ADD;
     const bool two_round = p.epi == LTXQ_EPI_GATE_THEN_ADD || p.gate.dtype == LTXQ_BF16;
     if (p.epi == LTXQ_EPI_GELU) {
@@ -201,17 +202,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!mbar_wait(&acc_full[buf], (it >> 1) & 1, abort_flag, p.err)) break;
       tc_fence_after();
       const uint32_t tacc = tmem + t_lane + static_cast<uint32_t>(buf * BN);
-      const int m = m0 + warp * 32 + lane;
+      const int m0w = m0 + q * 32;  // first token of this warp
 #pragma unroll 1
-      for (int c = 0; c < BN / 32; ++c) {
+      for (int c = warp >> 2; c < BN / 32; c += 2) {
         if (n0 + c * 32 >= p.N) break;  // uniform
         uint32_t v[32];
         tmem_ld_32x32b_x32(tacc + c * 32, v);
         tmem_wait_ld();
         if (sp >= 0) {  // fp32 partial, tile-local [token][feature]
           float* dst = p.partial + (static_cast<size_t>((u - dp) / splits) * splits + sp) * (2 * BM * BN) +
-                       (static_cast<int>(rank) * BM + warp * 32 + lane) * BN + c * 32;
-          if (m < p.M) {
+                       (static_cast<int>(rank) * BM + q * 32 + lane) * BN + c * 32;
+          if (m0w + lane < p.M) {
 #pragma unroll
             for (int j = 0; j < 32; j += 4)
               *reinterpret_cast<float4*>(dst + j) =
@@ -220,7 +221,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           continue;
         }
-        gemm::epi_row32(p, p.alpha, v, m, n0 + c * 32, gated, two_round, gtab);
+        uint32_t u8[4][4];
+        gemm::epi_pack32(p.alpha, v, u8);
+        gemm::epi_rows32(p, u8, m0w, n0 + c * 32, gated, two_round, gtab);
       }
       tc_fence_before();
       gemm::named_bar_sync(1, 32 * kEpiWarps);

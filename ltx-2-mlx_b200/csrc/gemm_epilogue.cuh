@@ -128,33 +128,70 @@ __device__ __forceinline__ void epi_row_store(const Params& p, uint32_t (&u)[4],
   *reinterpret_cast<uint4*>(p.out + off) = make_uint4(u[0], u[1], u[2], u[3]);
 }
 
-// Epilogue of 32 consecutive features [n0, n0 + 32) of token m, the fp32
-// accumulators in v (tokens on the TMEM lanes: a thread has a row): alpha, the
-// first rounding point, bias, GELU and the gated residual, 16-byte stores.
-__device__ __forceinline__ void epi_row32(const Params& p, float alpha, const uint32_t (&v)[32], int m, int n0, bool gated,
-                                          bool two_round, const uint16_t* gtab) {
-  const float zero8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+// Rows and pieces of a lane quad: lane j holds piece k of row j in u[k], and
+// then piece j of row i in u[i].
+__device__ __forceinline__ void quad_transpose(uint32_t (&u)[4][4]) {
+  const int j = threadIdx.x & 3;
 #pragma unroll
-  for (int k8 = 0; k8 < 4; ++k8) {
-    const int nf = n0 + k8 * 8;
-    if (nf >= p.N) break;  // uniform
-    uint32_t u[4];
+  for (int step = 1; step <= 2; ++step) {
+    const bool up = j & step;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      u[j] = pack_bf16x2(__fmul_rn(__uint_as_float(v[k8 * 8 + 2 * j]), alpha),
-                         __fmul_rn(__uint_as_float(v[k8 * 8 + 2 * j + 1]), alpha));
-    if (p.bias != nullptr) {
-      const uint4 bv = __ldg(reinterpret_cast<const uint4*>(p.bias + nf));
-      const uint32_t bw[4] = {bv.x, bv.y, bv.z, bv.w};
+    for (int k = 0; k < 2; ++k) {
+      const int lo = step == 1 ? 2 * k : k, hi = lo + step;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        u[j] = pack_bf16x2(__fadd_rn(lo_bf16(u[j]), lo_bf16(bw[j])), __fadd_rn(hi_bf16(u[j]), hi_bf16(bw[j])));
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t r = __shfl_xor_sync(0xffffffffu, up ? u[lo][w] : u[hi][w], step);
+        if (up) u[lo][w] = r;
+        else u[hi][w] = r;
+      }
     }
-    if (p.epi == LTXQ_EPI_GELU) {
+  }
+}
+
+// 32 accumulators of a token times alpha, rounded to bf16 (the first rounding
+// point), as four 16-byte pieces
+__device__ __forceinline__ void epi_pack32(float alpha, const uint32_t (&v)[32], uint32_t (&u)[4][4]) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) u[j] = gelu_tab_x2(u[j], gtab);
-    }
-    if (m < p.M) epi_row_store(p, u, m, nf, zero8, gated, two_round, false);
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      u[k][w] = pack_bf16x2(__fmul_rn(__uint_as_float(v[8 * k + 2 * w]), alpha),
+                            __fmul_rn(__uint_as_float(v[8 * k + 2 * w + 1]), alpha));
+}
+
+// Epilogue of 32 features [n0, n0 + 32) of a warp's 32 tokens [m0, m0 + 32),
+// lane = token, u as epi_pack32 leaves it: lane quads exchange 16-byte pieces,
+// so that each store writes 64 contiguous bytes of 8 rows (a store of one piece
+// of 32 rows takes four times the cycles: 9216 x 4096 x 16384 fp4 products 356
+// us with those, 313 without); bias, GELU and the gated residual on that side.
+__device__ __forceinline__ void epi_rows32(const Params& p, uint32_t (&u)[4][4], int m0, int n0, bool gated,
+                                           bool two_round, const uint16_t* gtab) {
+  const int lane = threadIdx.x & 31;
+  quad_transpose(u);
+  const int nf = n0 + 8 * (lane & 3);
+  if (nf >= p.N) return;
+  if (p.bias != nullptr) {
+    const uint4 bv = __ldg(reinterpret_cast<const uint4*>(p.bias + nf));
+    const uint32_t bw[4] = {bv.x, bv.y, bv.z, bv.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        u[i][w] = pack_bf16x2(__fadd_rn(lo_bf16(u[i][w]), lo_bf16(bw[w])), __fadd_rn(hi_bf16(u[i][w]), hi_bf16(bw[w])));
+  }
+  if (p.epi == LTXQ_EPI_GELU) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) u[i][w] = gelu_tab_x2(u[i][w], gtab);
+  }
+  const bool gate_bcast = p.gate.rows_per_vec == 0;
+  float g8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (gated && gate_bcast) load_vec8(p.gate, vec_row(p.gate, 0), nf, g8);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int m = m0 + (lane & ~3) + i;
+    if (m < p.M) epi_row_store(p, u[i], m, nf, g8, gated, two_round, gate_bcast);
   }
 }
 

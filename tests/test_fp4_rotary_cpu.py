@@ -134,9 +134,12 @@ def test_fp4_workspace_sizes(lib):
     from ltxq import _lib
 
     q = _lib.QWeight(16, 16, None, None, 4096, 2080, _lib.NVFP4, 4, 16, 0, 0, _lib.COMPUTE_FP4, 16, 1.0)
-    need = lib.ltxq_qlinear_workspace_size(9, ctypes.byref(q))
-    assert need >= 9 * 2080 // 2 + 9 * 4 * 512
-    assert lib.ltxq_adaln_qlinear_workspace_size(9, ctypes.byref(q)) >= need + 9 * 2080 * 2
+    need = lib.ltxq_qlinear_workspace_size(40, ctypes.byref(q))
+    assert need >= 40 * 2080 // 2 + 9 * 4 * 512
+    assert lib.ltxq_adaln_qlinear_workspace_size(40, ctypes.byref(q)) >= need + 40 * 2080 * 2
+    assert lib.ltxq_qlinear_workspace_size(9, ctypes.byref(q)) == 0  # a few rows are quantized as they are read
+    q.compute = _lib.COMPUTE_DEQUANT
+    assert lib.ltxq_qlinear_workspace_size(2048, ctypes.byref(q)) >= 4096 * 2080 * 2
     assert lib.ltxq_qlinear_workspace_size(0, ctypes.byref(q)) == 0
 
 
