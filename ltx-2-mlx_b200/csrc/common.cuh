@@ -10,6 +10,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 
 #include "ltxq.h"  // include/ (on the -I path)
@@ -37,6 +38,25 @@ int num_sms();
 // addresses are keyed by it, so that an address looked up in one context is
 // never used after the device is reset and a new context loads the module.
 void* current_cu_context();
+
+// A kernel's dynamic shared-memory limit, set once per device and context (a
+// call costs about half a microsecond) and again after a device reset.
+struct SmemAttr {
+  std::atomic<void*> done[64] = {};
+  ltxq_status set(const void* kernel, size_t bytes) {
+    int dev = 0;
+    if (ltxq_status st = cuda_check(cudaGetDevice(&dev), "cudaGetDevice")) return st;
+    void* ctx = current_cu_context();
+    const bool known = dev >= 0 && dev < 64;
+    if (known && ctx && done[dev].load(std::memory_order_acquire) == ctx) return LTXQ_OK;
+    if (ltxq_status st = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                         static_cast<int>(bytes)),
+                                    "smem attribute"))
+      return st;
+    if (known) done[dev].store(current_cu_context(), std::memory_order_release);
+    return LTXQ_OK;
+  }
+};
 
 // Device error word (bounded waits that expire write a code here); kernels
 // receive its address as a parameter.

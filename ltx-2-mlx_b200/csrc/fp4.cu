@@ -24,30 +24,33 @@ namespace fp4 {
 
 // ---------------------------------------------------------------- quantize / read back
 
-// One thread per 16 elements of a row; memory-bound (2 bytes read, 0.53 to
-// 0.56 written per element).  kAtomsOut: rows run over whole K stages, whose
-// groups past the row's end get scale 0 (the GEMM reads their codes as zeros);
-// otherwise scales go row-major.
+// Both ways: one thread per 16 elements of a row, memory-bound (2 bytes of
+// values and 0.53 to 0.56 of codes and scales per element).  A CTA's 256 threads
+// take a row side by side (width a power of two, 16 to 256: several short rows
+// per CTA, a long one in steps), so that no index is divided out: with a flat
+// 64-bit index 16384 x 4096 took 35 us to quantize.
+
+// kAtomsOut: rows run over whole K stages, whose groups past the row's end get
+// scale 0 (the GEMM reads their codes as zeros); otherwise scales go row-major.
 template <int F, bool kAtomsOut, bool kDiv>
-__global__ void __launch_bounds__(256) quantize_kernel(const uint16_t* __restrict__ x, int64_t rows, int64_t K,
-                                                       int64_t row_stride, float g, uint8_t* __restrict__ codes,
-                                                       uint8_t* __restrict__ scales) {
+__global__ void __launch_bounds__(256) quantize_kernel(const uint16_t* __restrict__ x, int64_t rows, int K,
+                                                       int64_t row_stride, float g, int log_width,
+                                                       uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   constexpr int kGroup = Traits<F>::kGroup;
-  const int64_t chunks = kAtomsOut ? (K + kStageK - 1) / kStageK * (kStageK / 16) : K / 16;
-  const int64_t total = rows * chunks;
+  const int chunks = kAtomsOut ? (K + kStageK - 1) / kStageK * (kStageK / 16) : K / 16;
   const int64_t row_tiles = (rows + 127) / 128;
   const float inv_g = F == kNv && !kDiv ? __frcp_rn(g) : 1.f;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  const int64_t rounds = (total + step - 1) / step;  // every lane takes part in the shuffles of every round
-  for (int64_t it = 0; it < rounds; ++it) {
-    const int64_t i = it * step + blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
-    const bool live = i < total;
-    const int64_t row = live ? i / chunks : 0;
-    const int64_t c = live ? i - row * chunks : 0;
+  const int width = 1 << log_width;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 >> log_width) + (threadIdx.x >> log_width);
+  const uint16_t* xr = x + row * row_stride;
+  uint8_t* cr = codes + row * (K / 2);
+  for (int c0 = 0; c0 < chunks; c0 += width) {  // every lane takes part in the shuffles of every step
+    const int c = c0 + (threadIdx.x & (width - 1));
+    const bool live = row < rows && c < chunks;
     const bool data = live && c * 16 < K;
     uint32_t u[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (data) {
-      const uint4* src = reinterpret_cast<const uint4*>(x + row * row_stride + c * 16);
+      const uint4* src = reinterpret_cast<const uint4*>(xr + c * 16);
       const uint4 a = __ldg(src), b = __ldg(src + 1);
       u[0] = a.x; u[1] = a.y; u[2] = a.z; u[3] = a.w;
       u[4] = b.x; u[5] = b.y; u[6] = b.z; u[7] = b.w;
@@ -61,9 +64,9 @@ __global__ void __launch_bounds__(256) quantize_kernel(const uint16_t* __restric
       const float a = __uint_as_float(am << 16);
       gs = nv_group(kDiv ? __fdiv_rn(a, g) : __fmul_rn(a, inv_g), am < 0x7F80u, inv_g);
     }
-    if (data) *reinterpret_cast<uint2*>(codes + row * (K / 2) + c * 8) = encode16<F, kDiv>(u, gs, g);
+    if (data) *reinterpret_cast<uint2*>(cr + c * 8) = encode16<F, kDiv>(u, gs, g);
     const uint32_t byte = data ? gs.byte : 0u;
-    const int64_t group = c * 16 / kGroup;
+    const int group = c * 16 / kGroup;
     if (kAtomsOut) {
       // four neighbouring groups are one word of an atom; a row starts at a multiple of 16 threads
       const int lane = threadIdx.x & 31;
@@ -85,22 +88,21 @@ __global__ void __launch_bounds__(256) quantize_kernel(const uint16_t* __restric
   }
 }
 
-// One thread per 16 elements: 8 bytes of codes and a scale in, 32 bytes out.
 template <int F, bool kAtomsIn>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ codes,
-                                                         const uint8_t* __restrict__ scales, int64_t rows, int64_t K,
-                                                         float g, uint16_t* __restrict__ out) {
+                                                         const uint8_t* __restrict__ scales, int64_t rows, int K,
+                                                         float g, int log_width, uint16_t* __restrict__ out) {
   constexpr int kGroup = Traits<F>::kGroup;
-  const int64_t chunks = K / 16;
-  const int64_t total = rows * chunks;
   const int64_t row_tiles = (rows + 127) / 128;
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t row = i / chunks, c = i - row * chunks;
-    const int64_t group = c * 16 / kGroup;
-    const uint2 w = __ldg(reinterpret_cast<const uint2*>(codes + row * (K / 2) + c * 8));
-    const uint32_t s2 = scale_bf16x2<F>(
-        __ldg(scales + (kAtomsIn ? atom_offset<F>(row, group, row_tiles) : row * (K / kGroup) + group)));
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 >> log_width) + (threadIdx.x >> log_width);
+  if (row >= rows) return;
+  const uint8_t* cr = codes + row * (K / 2);
+  const uint8_t* sr = scales + row * (K / kGroup);
+  uint16_t* orow = out + row * K;
+  for (int c = threadIdx.x & ((1 << log_width) - 1); c < K / 16; c += 1 << log_width) {
+    const int group = c * 16 / kGroup;
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(cr + c * 8));
+    const uint32_t s2 = scale_bf16x2<F>(kAtomsIn ? __ldg(scales + atom_offset<F>(row, group, row_tiles)) : __ldg(sr + group));
     uint32_t a[4], b[4];
     decode_word(w.x, s2, a);
     decode_word(w.y, s2, b);
@@ -111,7 +113,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
         b[k] = pack_bf16x2(__fmul_rn(lo_bf16(b[k]), g), __fmul_rn(hi_bf16(b[k]), g));
       }
     }
-    uint4* dst = reinterpret_cast<uint4*>(out + row * K + c * 16);
+    uint4* dst = reinterpret_cast<uint4*>(orow + c * 16);
     dst[0] = make_uint4(a[0], a[1], a[2], a[3]);
     dst[1] = make_uint4(b[0], b[1], b[2], b[3]);
   }
@@ -129,6 +131,18 @@ __global__ void __launch_bounds__(256) pack_scales_kernel(const uint8_t* __restr
     const int64_t row = i / Gp, gi = i - row * Gp;
     out[atom_offset<F>(row, gi, row_tiles)] = row < N && gi < G ? s[row * G + gi] : uint8_t(0);
   }
+}
+
+// a row's threads, as a power of two from 16 to 256, and the CTAs of that
+struct RowGrid {
+  int log_width;
+  unsigned grid;
+};
+static RowGrid row_grid(int64_t rows, int64_t chunks) {
+  int lw = 4;
+  while (lw < 8 && (1 << lw) < chunks) ++lw;
+  const int64_t per = 256 >> lw;
+  return RowGrid{lw, static_cast<unsigned>((rows + per - 1) / per)};
 }
 
 static unsigned grid_for(int64_t work) {
@@ -158,24 +172,28 @@ ltxq_status fp4_global_scale(int32_t mode, float g, float* out, const char* what
   return LTXQ_OK;
 }
 
-// The weight cache's row-major form (the caller checked the descriptor).
+// The weight cache's row-major form (the caller checked the descriptor, sizes below 2^30).
 ltxq_status launch_fp4_quantize_rows(const uint16_t* x, int64_t R, int64_t L, int32_t mode, float g, uint8_t* codes,
                                      uint8_t* scales, cudaStream_t s) {
-  const unsigned grid = fp4::grid_for(R * (L / 16));
+  const fp4::RowGrid r = fp4::row_grid(R, L / 16);
+  const int K = static_cast<int>(L);
   if (mode == LTXQ_MXFP4)
-    fp4::quantize_kernel<fp4::kMx, false, false><<<grid, 256, 0, s>>>(x, R, L, L, g, codes, scales);
+    fp4::quantize_kernel<fp4::kMx, false, false><<<r.grid, 256, 0, s>>>(x, R, K, L, g, r.log_width, codes, scales);
   else if (fp4::power_of_two(g))
-    fp4::quantize_kernel<fp4::kNv, false, false><<<grid, 256, 0, s>>>(x, R, L, L, g, codes, scales);
+    fp4::quantize_kernel<fp4::kNv, false, false><<<r.grid, 256, 0, s>>>(x, R, K, L, g, r.log_width, codes, scales);
   else
-    fp4::quantize_kernel<fp4::kNv, false, true><<<grid, 256, 0, s>>>(x, R, L, L, g, codes, scales);
+    fp4::quantize_kernel<fp4::kNv, false, true><<<r.grid, 256, 0, s>>>(x, R, K, L, g, r.log_width, codes, scales);
   return launch_check("fp4 quantize launch");
 }
 
 ltxq_status launch_fp4_dequantize_rows(const uint8_t* codes, const uint8_t* scales, int64_t R, int64_t L, int32_t mode,
                                        float g, uint16_t* out, cudaStream_t s) {
-  const unsigned grid = fp4::grid_for(R * (L / 16));
-  if (mode == LTXQ_MXFP4) fp4::dequantize_kernel<fp4::kMx, false><<<grid, 256, 0, s>>>(codes, scales, R, L, g, out);
-  else fp4::dequantize_kernel<fp4::kNv, false><<<grid, 256, 0, s>>>(codes, scales, R, L, g, out);
+  const fp4::RowGrid r = fp4::row_grid(R, L / 16);
+  const int K = static_cast<int>(L);
+  if (mode == LTXQ_MXFP4)
+    fp4::dequantize_kernel<fp4::kMx, false><<<r.grid, 256, 0, s>>>(codes, scales, R, K, g, r.log_width, out);
+  else
+    fp4::dequantize_kernel<fp4::kNv, false><<<r.grid, 256, 0, s>>>(codes, scales, R, K, g, r.log_width, out);
   return launch_check("fp4 dequantize launch");
 }
 
@@ -564,9 +582,8 @@ static ltxq_status launch_pair(const ltxq_fp4_act& x, const ltxq_qweight& w, con
                                       128, 2 * PL::AP, CU_TENSOR_MAP_SWIZZLE_NONE))
     return st;
   auto kern = qgemm_fp4_pair_kernel<F, kBlocks, BN>;
-  if (ltxq_status st = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PL::kSmem),
-                                  "smem attribute"))
-    return st;
+  static SmemAttr attr_done;
+  if (ltxq_status st = attr_done.set(reinterpret_cast<const void*>(kern), PL::kSmem)) return st;
   const int tiles = ((p.M + 2 * kBlocks * BM - 1) / (2 * kBlocks * BM)) * ((p.N + BN - 1) / BN);
   const int max_clusters = num_sms() / 2;
   const int clusters = tiles < max_clusters ? tiles : max_clusters;
@@ -631,16 +648,17 @@ ltxq_status launch_qlinear_fp4(const ltxq_fp4_act& x, int64_t M, const ltxq_qwei
 
 ltxq_status launch_fp4_quantize(const void* x, int64_t M, int64_t K, int64_t row_stride, const ltxq_fp4_act& o, float g,
                                 cudaStream_t s) {
-  const unsigned grid = fp4::grid_for(M * ((K + fp4::kStageK - 1) / fp4::kStageK) * (fp4::kStageK / 16));
+  const fp4::RowGrid r = fp4::row_grid(M, (K + fp4::kStageK - 1) / fp4::kStageK * (fp4::kStageK / 16));
   auto* src = static_cast<const uint16_t*>(x);
   auto* c = static_cast<uint8_t*>(o.codes);
   auto* sc = static_cast<uint8_t*>(o.scales);
+  const int k = static_cast<int>(K);
   if (o.mode == LTXQ_MXFP4)
-    fp4::quantize_kernel<fp4::kMx, true, false><<<grid, 256, 0, s>>>(src, M, K, row_stride, g, c, sc);
+    fp4::quantize_kernel<fp4::kMx, true, false><<<r.grid, 256, 0, s>>>(src, M, k, row_stride, g, r.log_width, c, sc);
   else if (fp4::power_of_two(g))
-    fp4::quantize_kernel<fp4::kNv, true, false><<<grid, 256, 0, s>>>(src, M, K, row_stride, g, c, sc);
+    fp4::quantize_kernel<fp4::kNv, true, false><<<r.grid, 256, 0, s>>>(src, M, k, row_stride, g, r.log_width, c, sc);
   else
-    fp4::quantize_kernel<fp4::kNv, true, true><<<grid, 256, 0, s>>>(src, M, K, row_stride, g, c, sc);
+    fp4::quantize_kernel<fp4::kNv, true, true><<<r.grid, 256, 0, s>>>(src, M, k, row_stride, g, r.log_width, c, sc);
   return launch_check("fp4 quantize launch");
 }
 
@@ -689,13 +707,15 @@ ltxq_status ltxq_fp4_dequantize(const ltxq_fp4_act* a, int64_t M, int64_t K, voi
   if (reinterpret_cast<uintptr_t>(out) & 15u) return fail(LTXQ_ERR_UNSUPPORTED, "fp4_dequantize: out not 16-byte aligned");
   if (M == 0) return LTXQ_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned grid = fp4::grid_for(M * (K / 16));
+  const fp4::RowGrid r = fp4::row_grid(M, K / 16);
+  const int k = static_cast<int>(K);
   auto* c = static_cast<const uint8_t*>(a->codes);
   auto* sc = static_cast<const uint8_t*>(a->scales);
+  auto* o = static_cast<uint16_t*>(out);
   if (a->mode == LTXQ_MXFP4)
-    fp4::dequantize_kernel<fp4::kMx, true><<<grid, 256, 0, s>>>(c, sc, M, K, g, static_cast<uint16_t*>(out));
+    fp4::dequantize_kernel<fp4::kMx, true><<<r.grid, 256, 0, s>>>(c, sc, M, k, g, r.log_width, o);
   else
-    fp4::dequantize_kernel<fp4::kNv, true><<<grid, 256, 0, s>>>(c, sc, M, K, g, static_cast<uint16_t*>(out));
+    fp4::dequantize_kernel<fp4::kNv, true><<<r.grid, 256, 0, s>>>(c, sc, M, k, g, r.log_width, o);
   return launch_check("fp4 dequantize launch");
 }
 

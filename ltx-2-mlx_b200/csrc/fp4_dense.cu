@@ -249,9 +249,8 @@ static ltxq_status launch(const void* x, const void* w, const gemm::Params& p, c
                                       BK, BN / 2, CU_TENSOR_MAP_SWIZZLE_128B))
     return st;
   auto kern = gemm_bf16_pair_kernel;
-  if (ltxq_status st = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PL::kSmem),
-                                  "smem attribute"))
-    return st;
+  static SmemAttr attr_done;
+  if (ltxq_status st = attr_done.set(reinterpret_cast<const void*>(kern), PL::kSmem)) return st;
   const int tiles = ((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + BN - 1) / BN);
   const int units = p.dp_tiles + (tiles - p.dp_tiles) * p.splits;
   const int max_clusters = num_sms() / 2;

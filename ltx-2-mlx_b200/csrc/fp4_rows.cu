@@ -283,9 +283,8 @@ constexpr size_t kRowSmem = 227 * 1024;
 template <int F, int kFill, int kNT>
 static ltxq_status launch_rows(const RowArgs& a, const gemm::Params& p, cudaStream_t stream) {
   auto kern = rows_kernel<F, kFill, kNT>;
-  if (ltxq_status st =
-          cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem), "smem attribute"))
-    return st;
+  static SmemAttr attr_done;
+  if (ltxq_status st = attr_done.set(reinterpret_cast<const void*>(kern), kRowSmem)) return st;
   const int tiles = (p.N + 15) / 16, sms = num_sms();
   kern<<<tiles < sms ? tiles : sms, kRowThreads, rows_smem(p.M, p.K), stream>>>(a, p);
   return launch_check("fp4 rows launch");

@@ -209,6 +209,7 @@ ltxq_status ltxq_quantize(const void* w_bf16, const ltxq_qweight* w, void* strea
   if (w->mode == LTXQ_MXFP4 || w->mode == LTXQ_NVFP4) {
     float g;
     if (ltxq_status st = fp4_global_scale(w->mode, w->global_scale, &g, "quantize")) return st;
+    if (R > 0x7FFFFFFF / 2 || L > 0x7FFFFFFF / 2) return fail(LTXQ_ERR_UNSUPPORTED, "quantize: dimension too large");
     if ((reinterpret_cast<uintptr_t>(w_bf16) | reinterpret_cast<uintptr_t>(w->weight)) & 15u)
       return fail(LTXQ_ERR_UNSUPPORTED, "quantize: the weight and its codes must be 16-byte aligned");
     return launch_fp4_quantize_rows(static_cast<const uint16_t*>(w_bf16), R, L, w->mode, g,
@@ -241,6 +242,7 @@ ltxq_status ltxq_dequantize(const ltxq_qweight* w, void* out_bf16, void* stream)
   if (w->mode == LTXQ_MXFP4 || w->mode == LTXQ_NVFP4) {
     float g;
     if (ltxq_status st = fp4_global_scale(w->mode, w->global_scale, &g, "dequantize")) return st;
+    if (R > 0x7FFFFFFF / 2 || L > 0x7FFFFFFF / 2) return fail(LTXQ_ERR_UNSUPPORTED, "dequantize: dimension too large");
     if (reinterpret_cast<uintptr_t>(w->weight) & 15u)
       return fail(LTXQ_ERR_UNSUPPORTED, "dequantize: the codes must be 16-byte aligned");
     return launch_fp4_dequantize_rows(static_cast<const uint8_t*>(w->weight), static_cast<const uint8_t*>(w->scales), R,

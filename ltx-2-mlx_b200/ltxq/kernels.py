@@ -165,21 +165,21 @@ class FP4Tensor:
     def __init__(self, rows_shape: tuple[int, ...], K: int, mode: str, device, global_scale: float = 1.0):
         if mode not in FP4_MODES:
             raise ValueError(f"mode must be one of {sorted(FP4_MODES)}, got {mode!r}")
+        if K <= 0 or K % 32 != 0:
+            raise ValueError(f"K must be a positive multiple of 32, got {K}")
+        if global_scale != 1.0:
+            if mode != "nvfp4":
+                raise ValueError("global_scale is nvfp4 only")
+            if not 2.0 ** -64 <= global_scale <= 2.0 ** 64:
+                raise ValueError("global_scale must be within [2^-64, 2^64]")
         self.rows_shape = tuple(rows_shape)
         self.K = int(K)
         self.mode = mode
         self.global_scale = float(global_scale)
-        self.M = math.prod(self.rows_shape)
-        if self.K <= 0 or self.K % 32 != 0:
-            raise ValueError(f"K must be a positive multiple of 32, got {self.K}")
-        group = 16 if mode == "nvfp4" else 32
-        if mode != "nvfp4" and self.global_scale != 1.0:
-            raise ValueError("global_scale is nvfp4 only")
-        if not 2.0 ** -64 <= self.global_scale <= 2.0 ** 64:
-            raise ValueError("global_scale must be within [2^-64, 2^64]")
+        self.M = M = math.prod(self.rows_shape)
         self._st = None
-        self._code_bytes = self.M * (self.K // 2)
-        self._scale_bytes = -(-self.K // 256) * -(-self.M // 128) * 128 * (256 // group)
+        self._code_bytes = M * (K // 2)
+        self._scale_bytes = (K + 255) // 256 * ((M + 127) // 128) * (2048 if mode == "nvfp4" else 1024)
         self._scale_off = _align(self._code_bytes)
         self.buffer = torch.empty(self._scale_off + self._scale_bytes, dtype=torch.uint8, device=device)
 
@@ -197,10 +197,11 @@ class FP4Tensor:
                 self.buffer[self._scale_off:self._scale_off + self._scale_bytes])
 
     def struct(self) -> _lib.Fp4Act:
-        if self._st is None:
+        st = self._st
+        if st is None:
             base = self.buffer.data_ptr()
-            self._st = _lib.Fp4Act(base, base + self._scale_off, FP4_MODES[self.mode], self.global_scale)
-        return self._st
+            st = self._st = _lib.Fp4Act(base, base + self._scale_off, FP4_MODES[self.mode], self.global_scale)
+        return st
 
     @classmethod
     def quantize(cls, x: torch.Tensor, mode: str = "nvfp4", global_scale: float = 1.0) -> "FP4Tensor":
@@ -233,7 +234,7 @@ class FP4Tensor:
         if dev != _device():
             with torch.cuda.device(dev):
                 return self.dequantize()
-        out = torch.empty(self.shape, dtype=torch.bfloat16, device=self.buffer.device)
+        out = self.buffer.new_empty(self.rows_shape + (self.K,), dtype=torch.bfloat16)
         if self.M:
             _lib.check(_lib.load().ltxq_fp4_dequantize(self.struct(), self.M, self.K, out.data_ptr(), _raw_stream(dev)),
                        "fp4_dequantize")
@@ -473,32 +474,36 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, heads:
     _require_cuda(x, "x")
     _require_cuda(positions, "positions")
     _require_cuda(freqs, "freqs")
-    if x.dtype not in _DT:
+    dt, shape, fshape, pshape = _DT.get(x.dtype), x.shape, freqs.shape, positions.shape
+    if dt is None:
         raise ValueError(f"x dtype must be bfloat16 or float32, got {x.dtype}")
     if layout not in _ROTARY_LAYOUT:
         raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
-    if heads <= 0 or x.dim() not in (3, 4) or (x.dim() == 4 and x.shape[2] != heads):
-        raise ValueError(f"x must be (B, T, {heads} * D) or (B, T, {heads}, D), got {tuple(x.shape)}")
-    if x.dim() == 3 and x.shape[2] % heads != 0:
+    four = len(shape) == 4
+    if heads <= 0 or not (four or len(shape) == 3) or (four and shape[2] != heads):
+        raise ValueError(f"x must be (B, T, {heads} * D) or (B, T, {heads}, D), got {tuple(shape)}")
+    if not four and shape[2] % heads != 0:
         raise ValueError("x's last dimension must be a multiple of heads")
-    b, t = x.shape[0], x.shape[1]
-    d = x.shape[3] if x.dim() == 4 else x.shape[2] // heads
-    if freqs.dtype != torch.float64 or freqs.dim() not in (1, 2) or (freqs.dim() == 2 and freqs.shape[0] != heads):
-        raise ValueError(f"freqs must be float64 (R/2,) or ({heads}, R/2), got {freqs.dtype} {tuple(freqs.shape)}")
-    r = 2 * freqs.shape[-1]
+    b, t = shape[0], shape[1]
+    d = shape[3] if four else shape[2] // heads
+    per_head = len(fshape) == 2
+    if freqs.dtype != torch.float64 or not (per_head or len(fshape) == 1) or (per_head and fshape[0] != heads):
+        raise ValueError(f"freqs must be float64 (R/2,) or ({heads}, R/2), got {freqs.dtype} {tuple(fshape)}")
+    r = 2 * fshape[-1]
     if r > d:
         raise ValueError(f"freqs rotate {r} elements but a head has {d}")
-    if positions.dtype not in _POS:
+    pos_type = _POS.get(positions.dtype)
+    if pos_type is None:
         raise ValueError(f"positions must be int32, int64, float32 or float64, got {positions.dtype}")
-    lead = positions.dim() - (1 if axes is None else 2)
-    if lead not in (0, 1) or positions.shape[-1] != t or (lead and positions.shape[0] != b):
-        raise ValueError(f"positions shape {tuple(positions.shape)} does not match {b} x {t} tokens")
+    lead = len(pshape) - (1 if axes is None else 2)
+    if lead not in (0, 1) or pshape[-1] != t or (lead and pshape[0] != b):
+        raise ValueError(f"positions shape {tuple(pshape)} does not match {b} x {t} tokens")
     n_axes = 1
     if axes is not None:
         _require_cuda(axes, "axes")
-        if axes.dtype != torch.int32 or axes.shape != freqs.shape:
+        if axes.dtype != torch.int32 or axes.shape != fshape:
             raise ValueError("axes must be int32 with the shape of freqs")
-        n_axes = positions.shape[-2]
+        n_axes = pshape[-2]
         axes = axes.contiguous()
         if n_axes < 1:
             raise ValueError("positions have no axis")
@@ -516,18 +521,17 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, heads:
             raise ValueError("an in-place rotation needs x with a unit last stride")
         x = x.contiguous()
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.shape != x.shape or out.dtype != x.dtype or (out.stride(-1) != 1 and out.shape[-1] > 1):
         raise ValueError("out must have x's shape and type and a unit last stride")
     if x.numel() == 0:
         return out
     freqs = freqs.contiguous()
     xs, os, ps = x.stride(), out.stride(), positions.stride()
-    four = len(xs) == 4
     args = _ROTARY_ARGS.pack(
-        x.data_ptr(), out.data_ptr(), _DT[x.dtype], _ROTARY_LAYOUT[layout], b, t, heads, d, r, xs[0], xs[1],
-        xs[2] if four else d, os[0], os[1], os[2] if four else d, positions.data_ptr(), ps[0] if lead else 0,
-        ps[-2] if axes is not None else 0, ps[-1], _POS[positions.dtype], n_axes, freqs.data_ptr(),
-        axes.data_ptr() if axes is not None else 0, freqs.dim() == 2, bool(inverse), scale, 0)
+        x.data_ptr(), out.data_ptr(), dt, _ROTARY_LAYOUT[layout], b, t, heads, d, r, xs[0], xs[1], xs[2] if four else d,
+        os[0], os[1], os[2] if four else d, positions.data_ptr(), ps[0] if lead else 0, ps[-2] if axes is not None else 0,
+        ps[-1], pos_type, n_axes, freqs.data_ptr(), axes.data_ptr() if axes is not None else 0, per_head, bool(inverse),
+        scale, 0)
     _lib.check(_lib.load().ltxq_rotary(args, _raw_stream(dev)), "rotary")
     return out

@@ -344,7 +344,7 @@ class QuantizedLinear:
             with torch.cuda.device(dev):
                 return self._call_fp4(x, gelu, residual, gate, gate_then_add, adaln, split_k)
         rows_shape = x.shape[:-1]
-        out = torch.empty((*rows_shape, self.out_features), dtype=torch.bfloat16, device=device)
+        out = (x.buffer if packed else x).new_empty((*rows_shape, self.out_features), dtype=torch.bfloat16)
         M = x.M if packed else x.numel() // self.in_features
         if M == 0:
             return out
@@ -366,7 +366,7 @@ class QuantizedLinear:
             ws_bytes = lib.ltxq_adaln_qlinear_workspace_size(M, q)
         else:
             ws_bytes = lib.ltxq_qlinear_workspace_size(M, q) if split_k or self.compute == "fp4" else 0
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
+        ws = out.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
         ws_ptr = ws.data_ptr() if ws is not None else None
         if pro is not None:
             _lib.check(lib.ltxq_adaln_qlinear(x.data_ptr(), M, pro, q, epi, out.data_ptr(), ws_ptr, ws_bytes, stream),
