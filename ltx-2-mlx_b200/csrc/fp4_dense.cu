@@ -4,9 +4,9 @@
 //
 // The fused kernel (qgemm.cu) converts every weight tile again for each 256
 // tokens, and its conversion warps, which feed the MMA through tensor memory,
-// bound it at 830 to 980 TFLOP/s.  From a few tiles of tokens on, converting
+// bound it at 780 to 1090 TFLOP/s.  From a few tiles of tokens on, converting
 // the weight once (2.5 bytes moved per element) and running both operands by
-// TMA costs less: 3456 x 4096 x 4096 takes the fused kernel 132 us.
+// TMA costs less: 3456 x 4096 x 4096 takes 91 us, the fused kernel 117.
 //
 // Persistent kernel, clusters of two CTAs (tcgen05 cta_group::2), tiles of 256
 // tokens x 256 features: CTA r holds token rows [m0 + 128 r, +128) (operand A,
@@ -281,8 +281,10 @@ size_t fp4_dense_bytes(int64_t M, const ltxq_qweight& w, size_t* partial_offset)
   if ((w.mode != LTXQ_MXFP4 && w.mode != LTXQ_NVFP4) || w.layout != LTXQ_LAYOUT_STD || w.compute == LTXQ_COMPUTE_FP4)
     return 0;
   if (w.n_out <= 0 || w.k_in <= 0 || w.k_in % 32 != 0) return 0;
-  // 768 tokens and 48 tiles: below, the conversion pass costs more than it saves (512 x 4096 x 4096: 40 us against 31;
-  // 1024 x 2048 x 2048, 32 tiles: 27 against 22; 768 x 4096 x 4096: 40 against 47, 3456 rows: 91 against 129)
+  // 768 tokens and 48 tiles: below, the conversion pass costs more than it saves (512 x 4096 x 4096: 36 us against the
+  // fused kernel's 28; 1024 x 2048 x 2048, 32 tiles: 26 against 21; 768 x 4096 x 4096: 37 against 43, 1536 x 2048 x
+  // 2048: 22 against 28, 3456 x 4096 x 4096: 91 against 117).  Wide outputs come out even at the limit (768 x 4096 x
+  // 16384: 109 against 108, 1024 rows: 129 against 126)
   if (M < 768 || (M + 255) / 256 * ((w.n_out + 255) / 256) < 48) return 0;
   const size_t weight = (static_cast<size_t>(w.n_out) * static_cast<size_t>(w.k_in) * 2 + 255) & ~size_t(255);
   if (partial_offset) *partial_offset = weight;

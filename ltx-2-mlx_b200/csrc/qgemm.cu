@@ -68,9 +68,9 @@ constexpr int kPrefetch = 2;      // scale/bias register prefetch distance (stag
 // kMxfp8F: mxfp8 data flagged LTXQ_QW_MXFP8_FINITE (short conversion)
 enum QKind { kAffine8 = 0, kAffine4 = 1, kMxfp8 = 2, kMxfp8F = 3, kMxfp4 = 4, kNvfp4 = 5 };
 constexpr bool is_fp4(int qk) { return qk == kMxfp4 || qk == kNvfp4; }
-// one byte per group and no biases; groups of 1 << group_log2 elements
-constexpr bool is_mx(int qk) { return qk == kMxfp8 || qk == kMxfp8F || is_fp4(qk); }
-constexpr int group_log2(int qk) { return qk == kNvfp4 ? 4 : 5; }
+constexpr bool is_mx(int qk) { return qk == kMxfp8 || qk == kMxfp8F; }
+// dequant warps that convert a stage (fp4: the others convert the next one)
+constexpr int stage_warps(int qk) { return is_fp4(qk) ? 4 : 8; }
 
 template <int QK>
 struct QTraits {
@@ -90,7 +90,7 @@ struct GroupCursor {
   uint4 cs, cb, ns, nb;
   // g0: the first group get() will be asked for
   __device__ __forceinline__ void init(const Params& p, int64_t srow, bool ok, int g0) {
-    const int gpr = is_mx(QK) ? p.K >> group_log2(QK) : p.K / p.gs;
+    const int gpr = is_mx(QK) ? p.K / 32 : p.K / p.gs;
     nblk = ok ? gpr / kPerBlk : 0;
     sb = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.scales) + srow * (is_mx(QK) ? 1 : 2));
     bb = is_mx(QK) ? nullptr : reinterpret_cast<const uint4*>(p.biases + srow);
@@ -117,7 +117,7 @@ struct GroupCursor {
     if (is_mx(QK)) {
       const int wi = e >> 2;
       const uint32_t w = wi == 0 ? cs.x : wi == 1 ? cs.y : wi == 2 ? cs.z : cs.w;
-      s = (w >> (8 * (e & 3))) & (QK == kNvfp4 ? 0xFFFFu : 0xFFu);
+      s = (w >> (8 * (e & 3))) & 0xFFu;
       b = 0u;
     } else {
       const int wi = e >> 1;
@@ -132,8 +132,7 @@ struct GroupCursor {
 
 // Group parameters of (row n, K-half starting at element k) as the packed
 // form the converters take: affine -> bf16x2 broadcast scale / bias;
-// mxfp8 / mxfp4 -> E8M0 byte in `s`; nvfp4 -> the E4M3 bytes of the half's two
-// groups.
+// mxfp8 -> E8M0 byte in `s`.
 template <int QK>
 __device__ __forceinline__ void load_group(const Params& p, int64_t row_off_scales, int k, bool ok, uint32_t& s,
                                            uint32_t& b) {
@@ -142,15 +141,7 @@ __device__ __forceinline__ void load_group(const Params& p, int64_t row_off_scal
     b = 0u;
     return;
   }
-  if (QK == kNvfp4) {
-    // two groups per K half: bytes, since a row's scales may start anywhere
-    const uint8_t* q = static_cast<const uint8_t*>(p.scales) + row_off_scales + (k >> 4);
-    s = k < p.K ? __ldg(q) | (static_cast<uint32_t>(__ldg(q + 1)) << 8) : 0u;
-    b = 0u;
-  } else if (QK == kMxfp4) {
-    s = k < p.K ? __ldg(static_cast<const uint8_t*>(p.scales) + row_off_scales + (k >> 5)) : 0u;
-    b = 0u;
-  } else if (is_mx(QK)) {
+  if (is_mx(QK)) {
     s = __ldg(static_cast<const uint8_t*>(p.scales) + row_off_scales + (k >> 5));
     b = 0u;
   } else {
@@ -225,14 +216,14 @@ __device__ __forceinline__ void dequant_loop(const Params& p, const Bars& bb, ui
   const int n = n0 + r;
   const bool row_ok = n < p.N;
   const uint32_t t_lane = static_cast<uint32_t>(q * 32) << 16;
-  const int64_t srow = static_cast<int64_t>(n) * (is_mx(QK) ? p.K >> group_log2(QK) : p.K / p.gs);
+  const int64_t srow = static_cast<int64_t>(n) * (is_mx(QK) ? p.K / 32 : p.K / p.gs);
   // group parameters of stage kb live in qs/qb[kb % kPrefetch]; the K loop
   // is unrolled by kPrefetch so every register is read kPrefetch stages
   // after its load was issued (no register moves that would wait on it)
   const bool vec = p.vec_groups != 0;
   const int k_first = kb_first * BK + half * 32;
   GroupCursor<QK> gc;
-  if (vec) gc.init(p, srow, row_ok, is_mx(QK) ? (k_first >> group_log2(QK)) : k_first / p.gs);
+  if (vec) gc.init(p, srow, row_ok, is_mx(QK) ? (k_first >> 5) : k_first / p.gs);
   uint32_t qs[kPrefetch], qb[kPrefetch];
 #pragma unroll
   for (int i = 0; i < kPrefetch; ++i)
@@ -263,7 +254,7 @@ __device__ __forceinline__ void dequant_loop(const Params& p, const Bars& bb, ui
       uint32_t s_cur = qs[i], b_cur = qb[i];
       if (vec) {
         const int k = k_first + kb * BK;
-        gc.get(is_mx(QK) ? (k >> group_log2(QK)) : k / p.gs, s_cur, b_cur);
+        gc.get(is_mx(QK) ? (k >> 5) : k / p.gs, s_cur, b_cur);
         if (!row_ok) {
           s_cur = 0u;
           b_cur = 0u;
@@ -286,32 +277,6 @@ __device__ __forceinline__ void dequant_loop(const Params& p, const Bars& bb, ui
           deq_affine4_word(wv[w4], s_cur, b_cur, q4);
 #pragma unroll
           for (int t = 0; t < 4; ++t) o[w4 * 4 + t] = q4[t];
-        }
-      } else if (is_fp4(QK)) {
-        // rows as for kAffine4; one scale per half (mxfp4) or per 16 elements (nvfp4)
-        const uint4 v = *reinterpret_cast<const uint4*>(wrow + ((half ^ ((r >> 2) & 1)) << 4));
-        const uint32_t wv[4] = {v.x, v.y, v.z, v.w};
-        constexpr int F = QK == kNvfp4 ? fp4::kNv : fp4::kMx;
-        bool fits;
-        uint32_t mul[2];
-        fp4::decode_mul2<F>(s_cur, mul, fits);
-        if (QK == kNvfp4 || __all_sync(0xffffffffu, fits)) {
-#pragma unroll
-          for (int w4 = 0; w4 < 4; ++w4) {
-            uint32_t q4[4];
-            fp4::decode_word1(wv[w4], mul[w4 >> 1], q4);
-#pragma unroll
-            for (int t = 0; t < 4; ++t) o[w4 * 4 + t] = q4[t];
-          }
-        } else {
-          const uint32_t s2 = fp4::scale_bf16x2<F>(s_cur);
-#pragma unroll
-          for (int w4 = 0; w4 < 4; ++w4) {
-            uint32_t q4[4];
-            fp4::decode_word(wv[w4], s2, q4);
-#pragma unroll
-            for (int t = 0; t < 4; ++t) o[w4 * 4 + t] = q4[t];
-          }
         }
       } else {
         // 64-byte rows, 64B swizzle: 16-byte chunk c sits at c ^ ((r >> 1) & 3);
@@ -351,6 +316,90 @@ __device__ __forceinline__ void dequant_loop(const Params& p, const Bars& bb, ui
     }
   }
   if (pend_as >= 0) publish(pend_as);
+}
+
+// The fp4 kinds' dequant warps: warps 0..3 (one per TMEM lane quarter) convert
+// the even stages, warps 4..7 the odd ones, a whole 64-wide row of a stage per
+// thread.  These kernels run few tokens (more of them take fp4_dense.cu), where
+// the MMA waits for each stage's chain of wait, convert, store and publish, so
+// two stages are in hand at once.  Against all eight warps on one stage (M x K
+// x N): mxfp4 201 x 2048 x 8192 19.8 us, was 20.7; nvfp4 767 x 16384 x 4096
+// 126, was 154; mxfp4 40 x 1056 x 2080 9.7, was 9.9.
+template <int QK, int S, int AS, uint32_t kACol>
+__device__ __forceinline__ void dequant_loop_fp4(const Params& p, const Bars& bb, uint8_t* ws, uint32_t tmem, int warp,
+                                                 int lane, int n0, int num_kb, uint32_t a_full_remote, int kb_base,
+                                                 int kb_first) {
+  // a warp meets a slot at every turn of its ring, so that a wait's parity names one phase
+  static_assert(S % 2 == 0 && AS % 2 == 0, "even rings");
+  constexpr int F = QK == kNvfp4 ? fp4::kNv : fp4::kMx;
+  constexpr int kGroup = fp4::Traits<F>::kGroup;
+  constexpr int kWStage = BM * QTraits<QK>::kWBytes;
+  const int q = warp & 3;
+  const int r = q * 32 + lane;  // feature row within the tile == TMEM lane
+  const int n = n0 + r;
+  const bool row_ok = n < p.N;
+  const uint8_t* sp = static_cast<const uint8_t*>(p.scales) + static_cast<int64_t>(row_ok ? n : 0) * (p.K / kGroup);
+  // a stage's scales of a row: one word (nvfp4) or half word (mxfp4) where rows are aligned so
+  const bool wide = p.K % 64 == 0 && (reinterpret_cast<uintptr_t>(p.scales) & (F == fp4::kNv ? 3u : 1u)) == 0;
+  auto scales = [&](int kb) -> uint32_t {
+    const int k = (kb_first + kb) * BK;
+    if (kb >= num_kb || !row_ok) return 0u;
+    if (wide)
+      return F == fp4::kNv ? __ldg(reinterpret_cast<const uint32_t*>(sp + k / kGroup))
+                           : __ldg(reinterpret_cast<const uint16_t*>(sp + k / kGroup));
+    uint32_t v = 0;
+#pragma unroll
+    for (int e = 0; e < BK / kGroup; ++e)
+      if (k + e * kGroup < p.K) v |= static_cast<uint32_t>(__ldg(sp + k / kGroup + e)) << (8 * e);
+    return v;
+  };
+  const int first = ((kb_base ^ (warp >> 2)) & 1);  // the stage at ring position kb_base + first is this warp's
+  uint32_t s0 = scales(first), s1 = scales(first + 2);
+  for (int kb = first; kb < num_kb; kb += 2) {
+    const int g = kb_base + kb;  // position in the smem / TMEM rings
+    const int s = g % S, as = g % AS;
+    const uint32_t sc = s0;
+    s0 = s1;
+    s1 = scales(kb + 4);
+    if (!mbar_wait(&bb.w_full[s], (g / S) & 1, bb.abort_flag, p.err)) return;
+    // 32-byte rows, 32B swizzle: 16-byte chunk c sits at c ^ ((r >> 2) & 1)
+    const uint8_t* wrow = ws + s * kWStage + r * QTraits<QK>::kWBytes;
+    uint32_t o[32];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 v = *reinterpret_cast<const uint4*>(wrow + ((h ^ ((r >> 2) & 1)) << 4));
+      const uint32_t wv[4] = {v.x, v.y, v.z, v.w};
+      const uint32_t sh = (F == fp4::kNv ? sc >> (16 * h) : sc >> (8 * h)) & (F == fp4::kNv ? 0xFFFFu : 0xFFu);
+      bool fits;
+      uint32_t mul[2];
+      fp4::decode_mul2<F>(sh, mul, fits);
+      const bool fast = F == fp4::kNv || __all_sync(0xffffffffu, fits);
+      const uint32_t s2 = fast ? 0u : fp4::scale_bf16x2<F>(sh);
+#pragma unroll
+      for (int w4 = 0; w4 < 4; ++w4) {
+        uint32_t q4[4];
+        fp4::decode_word1(wv[w4], fast ? mul[w4 >> 1] : 0x7E807E80u, q4);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          if (F == fp4::kMx && !fast) q4[t] = fma_bf16x2(q4[t], s2, 0x80008000u);  // a scale above 2: 2^126 and it apart
+          o[h * 16 + w4 * 4 + t] = row_ok ? q4[t] : 0u;
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bb.w_empty[s]);  // packed bytes consumed
+    if (!mbar_wait(&bb.a_empty[as], ((g / AS) & 1) ^ 1, bb.abort_flag, p.err)) return;
+    const uint32_t dst = tmem + (static_cast<uint32_t>(q * 32) << 16) + kACol + as * 32;
+    tmem_st_32x32b_x16(dst, o);
+    tmem_st_32x32b_x16(dst + 16, o + 16);
+    tmem_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) {
+      if (a_full_remote) mbar_arrive_cluster(a_full_remote + 8u * static_cast<uint32_t>(as));
+      else mbar_arrive(&bb.a_full[as]);
+    }
+  }
 }
 
 // An accumulator's value: nvfp4 weights enter as code * scale * kDecodeScale
@@ -451,10 +500,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bb.x_full[s], 1);
       mbar_init(&bb.x_empty[s], 1);
       mbar_init(&bb.w_full[s], 1);
-      mbar_init(&bb.w_empty[s], kDeqWarps);
+      mbar_init(&bb.w_empty[s], stage_warps(QK));
     }
     for (int s = 0; s < AS; ++s) {
-      mbar_init(&bb.a_full[s], kDeqWarps);
+      mbar_init(&bb.a_full[s], stage_warps(QK));
       mbar_init(&bb.a_empty[s], 1);
     }
     mbar_init(bb.acc_full, 1);
@@ -527,7 +576,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    dequant_loop<QK, S, AS, P::kACol>(p, bb, ws, tmem, warp, lane, n0, num_kb, 0u, 0, 0);
+    if constexpr (is_fp4(QK)) dequant_loop_fp4<QK, S, AS, P::kACol>(p, bb, ws, tmem, warp, lane, n0, num_kb, 0u, 0, 0);
+    else dequant_loop<QK, S, AS, P::kACol>(p, bb, ws, tmem, warp, lane, n0, num_kb, 0u, 0, 0);
     if (!*bb.abort_flag && mbar_wait(bb.acc_full, 0, bb.abort_flag, p.err)) {
       tc_fence_after();
       epilogue<QK, BN>(p, xs, tmem, warp, lane, n0, m0);
@@ -722,10 +772,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       mbar_init(&bb.x_full[s], 1);
       mbar_init(&bb.x_empty[s], 1);
       mbar_init(&bb.w_full[s], 1);
-      mbar_init(&bb.w_empty[s], kDeqWarps);
+      mbar_init(&bb.w_empty[s], stage_warps(QK));
     }
     for (int s = 0; s < AS; ++s) {
-      mbar_init(&bb.a_full[s], 2 * kDeqWarps);  // both CTAs' dequant warps (the leader's copy is used)
+      mbar_init(&bb.a_full[s], 2 * stage_warps(QK));  // both CTAs' dequant warps (the leader's copy is used)
       mbar_init(&bb.a_empty[s], 1);
     }
     mbar_init(bb.acc_full, 1);
@@ -830,7 +880,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     for (int u = cluster_id; u < units && !*bb.abort_flag; u += n_clusters) {
       int n0, m0, sp, kb_lo, kb_hi;
       unit(u, n0, m0, sp, kb_lo, kb_hi);
-      dequant_loop<QK, S, AS, P::kACol>(p, bb, ws, tmem, warp, lane, n0, kb_hi - kb_lo, leader_a_full, g0, kb_lo);
+      if constexpr (is_fp4(QK))
+        dequant_loop_fp4<QK, S, AS, P::kACol>(p, bb, ws, tmem, warp, lane, n0, kb_hi - kb_lo, leader_a_full, g0, kb_lo);
+      else
+        dequant_loop<QK, S, AS, P::kACol>(p, bb, ws, tmem, warp, lane, n0, kb_hi - kb_lo, leader_a_full, g0, kb_lo);
       g0 += kb_hi - kb_lo;
     }
   } else {
