@@ -428,8 +428,11 @@ def _cat_linears(parts: list[QuantizedLinear]) -> QuantizedLinear:
     """Concatenate quantized linears along the output dimension.  Exact: in the
     standard layout each packed row keeps its own groups; in the pretransposed
     layout (groups along the output dimension) every part's width is a whole
-    number of groups, so its columns keep theirs."""
+    number of groups, so its columns keep theirs.  A fused weight has one
+    tensor scale, so nvfp4 parts of different ones are refused."""
     p0 = parts[0]
+    if any(p.global_scale != p0.global_scale for p in parts):
+        raise ValueError("projections that are fused into one GEMM need the same global_scale")
     for p in parts[1:]:
         assert p.in_features == p0.in_features and p.mode == p0.mode and p.bits == p0.bits
         assert p.group_size == p0.group_size and p.pretransposed == p0.pretransposed
@@ -444,7 +447,7 @@ def _cat_linears(parts: list[QuantizedLinear]) -> QuantizedLinear:
         torch.cat([p.weight for p in parts], dim), torch.cat([p.scales for p in parts], dim),
         torch.cat([p.biases for p in parts], dim) if p0.biases is not None else None, bias,
         group_size=p0.group_size, bits=p0.bits, mode=p0.mode, pretransposed=p0.pretransposed,
-        in_features=p0.in_features, out_features=sum(p.out_features for p in parts))
+        in_features=p0.in_features, out_features=sum(p.out_features for p in parts), global_scale=p0.global_scale)
 
 
 class BasicAVTransformerBlock:
@@ -517,7 +520,7 @@ class BasicAVTransformerBlock:
     def set_compute(self, compute: str) -> "BasicAVTransformerBlock":
         """How every quantized GEMM of the block computes (``QuantizedLinear.
         set_compute``): "dequant", or "mx2" / "mx1" for the native block-scaled
-        fp8 MMAs on mxfp8 weights."""
+        fp8 MMAs on mxfp8 weights, or "fp4" for those on mxfp4 / nvfp4 weights."""
         for ql in self.quantized_modules():
             ql.set_compute(compute)
         return self

@@ -11,7 +11,8 @@ Format (LTX_2_MLX/loader/transformer_cache.py):
   :113-125);
 * quantized block linears (``_CACHE_QUANTIZED_BLOCK_LINEAR_BASES`` :35-59)
   are stored as ``__quant__.transformer_blocks.{i}.{base}.weight`` (uint32
-  packed codes), ``.scales`` (bf16 for affine, uint8 E8M0 for mxfp8) and,
+  packed codes), ``.scales`` (bf16 for affine, uint8 E8M0 for mxfp8
+  and mxfp4, uint8 E4M3 for nvfp4) and,
   for affine only, ``.biases`` (:1255-1267); the linear's bias stays
   unquantized under its plain key ``transformer_blocks.{i}.{base}.bias``;
 * every other parameter keeps its plain MLX key, e.g.
@@ -55,6 +56,7 @@ SHARD_LIMIT_BYTES = 4 * 1024 ** 3
 CACHE_SCHEMA_VERSION = 1
 QUANTIZE_OFF, QUANTIZE_MXFP8_BLOCKS, QUANTIZE_MXFP8_BLOCKS_PRETRANSPOSE = (
     "off", "mxfp8-blocks", "mxfp8-blocks-pretranspose")
+FP4_GROUPS = {"mxfp4": 32, "nvfp4": 16}  # 4-bit floating point formats: values per scale
 ATTENTION_MODULES = ("attn1", "attn2", "audio_attn1", "audio_attn2", "audio_to_video_attn", "video_to_audio_attn")
 ATTENTION_PROJECTIONS = ("to_q", "to_k", "to_v", "to_out", "to_gate_logits")
 QUANTIZED_BLOCK_LINEAR_BASES = tuple(f"{m}.{p}" for m in ATTENTION_MODULES for p in ATTENTION_PROJECTIONS) + (
@@ -365,7 +367,8 @@ def quantized_linears_from_state(state: dict, in_features: dict[str, int], paylo
                                  mode: str | None = None, group_size: int | None = None,
                                  bits: int | None = None) -> dict:
     """``QuantizedLinear`` per base of one block's cache state.  The mode
-    comes from the scales' dtype (uint8 E8M0 -> mxfp8, bf16 -> affine)
+    comes from the scales' dtype (bf16 -> affine; uint8 -> mxfp8, or, where
+    a row packs 4 bits a value, mxfp4 / nvfp4 by its 32 / 16 values a scale)
     unless given; group size and bits from the payload overrides or the
     reference's per-mode defaults (affine 64/4, mxfp8 32/8); ``in_features``
     maps base -> K (the packed arrays alone leave bits x K ambiguous)."""
@@ -375,9 +378,13 @@ def quantized_linears_from_state(state: dict, in_features: dict[str, int], paylo
     pretransposed = payload.get("transformer_cache_quantize") == QUANTIZE_MXFP8_BLOCKS_PRETRANSPOSE
     out = {}
     for base, arrs in state["quant"].items():
-        m = mode or ("mxfp8" if arrs["scales"].dtype == torch.uint8 else "affine")
         k = in_features[base]
         rows, cols = arrs["weight"].shape
+        m = mode or ("mxfp8" if arrs["scales"].dtype == torch.uint8 else "affine")
+        if mode is None and m == "mxfp8" and not pretransposed and cols * 8 == k:
+            m = next((f for f, g in FP4_GROUPS.items() if arrs["scales"].shape[1] * g == k), None)
+            if m is None:
+                raise ValueError(f"{base}: {arrs['scales'].shape[1]} scales for {k} values in 4 bits")
         if not pretransposed and bits is None and (cols * 32) % k == 0:
             bits_b = cols * 32 // k  # packed along K: the row length fixes the bit width
         else:

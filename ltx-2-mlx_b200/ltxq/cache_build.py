@@ -28,6 +28,9 @@ Beyond the reference's modes (off, mxfp8-blocks, mxfp8-blocks-pretranspose),
 ``affine=(bits, group_size)`` quantizes the block linears with MLX affine
 int8 / int4 (the layout of benchmark configs 1-3 and 5); the payload then
 records ``block_linear_quantize = "affine"`` with its bits and group size.
+``fp4="mxfp4"`` / ``"nvfp4"`` quantizes them to 4-bit floating point and
+records that format the same way (nvfp4 without a tensor scale: the
+reference's arrays have no place for one).
 """
 
 from __future__ import annotations
@@ -101,17 +104,24 @@ def _block_linear(mlx_key: str):
 
 def build_transformer_cache(checkpoint, cache_file, mode: str = C.QUANTIZE_MXFP8_BLOCKS,
                             affine: tuple[int, int] | None = None, include_audio: bool = True,
-                            device="cuda", shard_limit_bytes: int = C.SHARD_LIMIT_BYTES) -> dict:
+                            device="cuda", shard_limit_bytes: int = C.SHARD_LIMIT_BYTES,
+                            fp4: str | None = None) -> dict:
     """Write the cache of ``checkpoint`` (a safetensors file with
     ``model.diffusion_model.`` keys) beside ``cache_file``; returns the
     metadata payload.  ``affine=(bits, group_size)`` quantizes the block
     linears affine instead of mxfp8 (no reference mode: the payload adds
-    ``block_linear_quantize`` keys)."""
+    ``block_linear_quantize`` keys); ``fp4="mxfp4"`` or ``"nvfp4"`` quantizes
+    them to that format, with the same keys."""
     from .quantized_linear import QuantizedLinear
 
     if affine is not None and mode != C.QUANTIZE_OFF:
         raise ValueError("affine block quantization goes with mode='off' (the reference's modes are mxfp8)")
-    quant = affine is not None or mode != C.QUANTIZE_OFF
+    if fp4 is not None:
+        if fp4 not in C.FP4_GROUPS:
+            raise ValueError(f"fp4 must be one of {sorted(C.FP4_GROUPS)}, got {fp4!r}")
+        if affine is not None or mode != C.QUANTIZE_OFF:
+            raise ValueError("fp4 block quantization goes with mode='off' and no affine")
+    quant = affine is not None or fp4 is not None or mode != C.QUANTIZE_OFF
     pretransposed = mode == C.QUANTIZE_MXFP8_BLOCKS_PRETRANSPOSE
     entries: dict[str, torch.Tensor] = {}
     for key, value in iter_checkpoint_weights(checkpoint, device):
@@ -128,6 +138,8 @@ def build_transformer_cache(checkpoint, cache_file, mode: str = C.QUANTIZE_MXFP8
         w = value.to(device=device, dtype=torch.bfloat16)
         if affine is not None:
             ql = QuantizedLinear.from_linear(w, None, group_size=affine[1], bits=affine[0], mode="affine")
+        elif fp4 is not None:
+            ql = QuantizedLinear.from_linear(w, None, mode=fp4)
         else:
             ql = QuantizedLinear.from_linear(w, None, mode="mxfp8", pretransposed=pretransposed)
         q = f"{C.QUANT_KEY_PREFIX}transformer_blocks.{i}.{base}"
@@ -140,6 +152,9 @@ def build_transformer_cache(checkpoint, cache_file, mode: str = C.QUANTIZE_MXFP8
     if affine is not None:
         payload.update(block_linear_quantize="affine", block_linear_quantize_bits=affine[0],
                        block_linear_quantize_group_size=affine[1])
+    if fp4 is not None:
+        payload.update(block_linear_quantize=fp4, block_linear_quantize_bits=4,
+                       block_linear_quantize_group_size=C.FP4_GROUPS[fp4])
     C.write_cache_weights(cache_file, entries, shard_limit_bytes)
     C.write_metadata(Path(cache_file).parent, payload)
     return payload

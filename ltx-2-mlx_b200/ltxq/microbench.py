@@ -33,7 +33,8 @@ DEFAULT_SHAPES = ["1024x4096x4096", "3456x4096x16384", "3456x16384x4096", "9216x
                   "9216x16384x4096", "126x2048x8192", "201x4096x2048"]
 # name -> (quantization mode, bits, compute mode)
 MODES = {"affine8": ("affine", 8, "dequant"), "affine4": ("affine", 4, "dequant"), "mxfp8": ("mxfp8", 8, "dequant"),
-         "mxfp8_mx2": ("mxfp8", 8, "mx2"), "mxfp8_mx1": ("mxfp8", 8, "mx1")}
+         "mxfp8_mx2": ("mxfp8", 8, "mx2"), "mxfp8_mx1": ("mxfp8", 8, "mx1"), "mxfp4": ("mxfp4", 4, "dequant"),
+         "nvfp4": ("nvfp4", 4, "dequant"), "mxfp4_fp4": ("mxfp4", 4, "fp4"), "nvfp4_fp4": ("nvfp4", 4, "fp4")}
 
 
 def _time(fn, flush, iters, warmup):
@@ -177,6 +178,7 @@ def main(argv=None):
                 qls = [ql] + [QuantizedLinear(ql.weight.clone(), ql.scales.clone(),
                                               None if ql.biases is None else ql.biases.clone(), ql.bias,
                                               group_size=ql.group_size, bits=ql.bits, mode=ql.mode,
+                                              global_scale=ql.global_scale,
                                               pretransposed=ql.pretransposed, in_features=ql.in_features,
                                               out_features=ql.out_features).set_compute(compute)
                               for _ in range(copies - 1)]

@@ -93,6 +93,9 @@ class QuantizedLinear:
             raise ValueError(f"unknown compute mode {compute!r}")
         self.compute = compute
         self._mx_scales = None
+        self._q4 = None
+        if getattr(self, "_fp4_packed", None) is not None:
+            self._fp4_packed = (None, 0, self._fp4_packed[2])  # packed again, in place
         if compute != "dequant":
             self.mx_scales()  # packed now, not inside a later stream capture
         return self
@@ -103,19 +106,7 @@ class QuantizedLinear:
         (``ltxq_fp4_pack_weight_scales``), made once and again only when the
         scale tensor changes; None where those modes do not apply."""
         if self.computes_fp4():
-            key = (self.scales.data_ptr(), _version(self.scales))
-            cached = getattr(self, "_mx_scales", None)
-            if cached is None or cached[0] != key:
-                with _on(self.scales):
-                    lib = _lib.load()
-                    q = self._qweight_base(0, None)
-                    buf = torch.empty(lib.ltxq_fp4_weight_scales_size(ctypes.byref(q)), dtype=torch.uint8,
-                                      device=self.scales.device)
-                    _lib.check(lib.ltxq_fp4_pack_weight_scales(ctypes.byref(q), buf.data_ptr(), _stream()),
-                               "fp4_pack_weight_scales")
-                cached = (key, buf)
-                self._mx_scales = cached
-            return cached[1]
+            return self._fp4_scales()
         if getattr(self, "compute", "dequant") in ("dequant", "fp4") or self.mode != "mxfp8" or self.pretransposed:
             return None
         if self.in_features % 512 != 0:
@@ -131,6 +122,27 @@ class QuantizedLinear:
             cached = (key, buf)
             self._mx_scales = cached
         return cached[1]
+
+    def _fp4_scales(self) -> torch.Tensor:
+        """The packed scales of "fp4".  They belong to one scale tensor (the
+        object, kept here) in one state: another tensor, or one changed in
+        place, is packed again by the next call or ``set_compute``, into the
+        same memory, which captured graphs read.  A graph replayed after such
+        a change therefore needs one of the two first.  Tensors made in
+        inference mode do not count their changes, so ``set_compute`` always
+        packs."""
+        scales, version, buf = getattr(self, "_fp4_packed", (None, 0, None))
+        if scales is not self.scales or version != _version(self.scales):
+            with _on(self.scales):
+                lib = _lib.load()
+                q = self._qweight_base(0, None)
+                nbytes = lib.ltxq_fp4_weight_scales_size(ctypes.byref(q))
+                if buf is None or buf.numel() != nbytes or buf.device != self.scales.device:
+                    buf = torch.empty(nbytes, dtype=torch.uint8, device=self.scales.device)
+                _lib.check(lib.ltxq_fp4_pack_weight_scales(ctypes.byref(q), buf.data_ptr(), _stream()),
+                           "fp4_pack_weight_scales")
+            self._fp4_packed = (self.scales, _version(self.scales), buf)
+        return buf
 
     def computes_fp4(self) -> bool:
         """Whether products over this weight are of two fp4 operands."""
@@ -310,11 +322,12 @@ class QuantizedLinear:
     def _qweight4(self) -> _lib.QWeight:
         """``qweight()`` of an fp4 weight, kept until one of its tensors or
         settings changes."""
-        key = (self.weight.data_ptr(), self.scales.data_ptr(), _version(self.scales),
+        key = (self.weight.data_ptr(), self.scales.data_ptr(), id(self.scales), _version(self.scales),
                self.bias.data_ptr() if self.bias is not None else 0, self.compute, self.global_scale)
         cached = getattr(self, "_q4", None)
+        # the scale tensor is kept, so that its id names no other one
         if cached is None or cached[0] != key:
-            cached = (key, self.qweight())
+            cached = (key, self.qweight(), self.scales)
             self._q4 = cached
         return cached[1]
 
