@@ -102,7 +102,10 @@ enum {
  *    to the weight's format (ltxq_fp4_quantize, global_scale 1) and the two
  *    quantized operands multiplied, at every M.  Needs the repacked weight
  *    scales (mx_scales from ltxq_fp4_pack_weight_scales) and the workspace
- *    that ltxq_qlinear_workspace_size returns; less is LTXQ_ERR_INVALID.
+ *    that ltxq_qlinear_workspace_size returns (none for the few rows of the
+ *    kernel that quantizes as it reads); less is LTXQ_ERR_INVALID.  nvfp4
+ *    activations past 6 * 448 in magnitude saturate: quantize those with a
+ *    global_scale of their own and call ltxq_qlinear_fp4.
  *    4-bit activations do not meet this path's stated tolerance against the
  *    reference (opt-in). */
 enum { LTXQ_COMPUTE_DEQUANT = 0, LTXQ_COMPUTE_MX2 = 1, LTXQ_COMPUTE_MX1 = 2, LTXQ_COMPUTE_FP4 = 3 };
@@ -251,8 +254,8 @@ ltxq_status ltxq_qk_norm_rope_pair(const void* q, const void* k, int64_t rows, i
  * (i, i + rotary_dim/2) in the half layout, (2i, 2i + 1) in the interleaved
  * one, i < rotary_dim/2; elements past rotary_dim pass through.  `inverse`
  * rotates back by the same angle with the same scale: the gradient of the
- * forward call.  Angles are reduced in fp64, the rotation is fp32, one rounding
- * to the output type.  An axis outside [0, n_axes) gives NaN. */
+ * forward call.  Angles are formed and reduced in two fp32 parts (in fp64 from
+ * 2^20 turns on), the rotation is fp32, one rounding to the output type.  An axis outside [0, n_axes) gives NaN. */
 enum { LTXQ_ROTARY_HALF = 0, LTXQ_ROTARY_INTERLEAVED = 1 };
 enum { LTXQ_POS_I32 = 0, LTXQ_POS_I64 = 1, LTXQ_POS_F32 = 2, LTXQ_POS_F64 = 3 };
 typedef struct {
@@ -399,7 +402,8 @@ ltxq_status ltxq_fp4_dequantize(const ltxq_fp4_act* a, int64_t M, int64_t K, voi
 size_t ltxq_fp4_weight_scales_size(const ltxq_qweight* w);
 ltxq_status ltxq_fp4_pack_weight_scales(const ltxq_qweight* w, void* out, void* stream);
 /* ltxq_qlinear from quantized activations of the weight's own format:
- * out = epilogue(dequant(x) . dequant(W)^T).  No workspace.  One quantized x
+ * out = epilogue(dequant(x) . dequant(W)^T).  No workspace.  The product of the
+ * global scales must be within [2^-96, 2^96].  One quantized x
  * serves every projection that reads it. */
 ltxq_status ltxq_qlinear_fp4(const ltxq_fp4_act* x, int64_t M, const ltxq_qweight* w, const ltxq_epilogue* epi,
                              void* out, void* stream);

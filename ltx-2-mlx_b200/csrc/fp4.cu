@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(Plan<F, kBlocks, BN>::kThreads, 1)
     }
     for (int b = 0; b < P::kAccBufs; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 2);
+      mbar_init(&acc_empty[b], 2 * P::kEpiWarps);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sf_ready[b], 8);  // four warps of each CTA
@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(Plan<F, kBlocks, BN>::kThreads, 1)
     for (int t = cluster_id; t < tiles && ok; t += n_clusters) {
       for (int kb = 0; kb < num_kb; ++kb, ++g) {
         const int s = g % S, sb = g & 1;
-        if (!mbar_wait(&sf_full[s], (g / S) & 1, abort_flag, p.err)) {
+        if (!mbar_wait_warp(&sf_full[s], (g / S) & 1, abort_flag, p.err)) {
           ok = false;
           break;
         }
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(Plan<F, kBlocks, BN>::kThreads, 1)
           const int c = P::kSfbOffCol + 8 * (i % AP) + 4 * (i / AP);
           r[c] = v.x; r[c + 1] = v.y; r[c + 2] = v.z; r[c + 3] = v.w;
         }
-        if (!mbar_wait(&sf_empty[sb], ((g >> 1) & 1) ^ 1, abort_flag, p.err)) {
+        if (!mbar_wait_warp(&sf_empty[sb], ((g >> 1) & 1) ^ 1, abort_flag, p.err)) {
           ok = false;
           break;
         }
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(Plan<F, kBlocks, BN>::kThreads, 1)
       int m0, n0;
       coords(t, m0, n0);
       const int buf = it % P::kAccBufs;
-      if (!mbar_wait(&acc_full[buf], (it / P::kAccBufs) & 1, abort_flag, p.err)) break;
+      if (!mbar_wait_warp(&acc_full[buf], (it / P::kAccBufs) & 1, abort_flag, p.err)) break;
       tc_fence_after();
       const uint32_t tacc = tmem + t_lane + static_cast<uint32_t>((kBlocks == 1 ? buf : blk) * BN);
       const int m0w = m0 + blk * BM + q * 32;  // first token of this warp
@@ -518,8 +518,8 @@ __global__ void __launch_bounds__(Plan<F, kBlocks, BN>::kThreads, 1)
         gemm::epi_rows32(p, u, m0w, n0 + c * 32, gated, two_round, gtab);
       }
       tc_fence_before();
-      gemm::named_bar_sync(1, 32 * P::kEpiWarps);
-      if (threadIdx.x == 0) mbar_arrive_cluster(leader_acc_empty + 8u * static_cast<uint32_t>(buf));
+      __syncwarp();  // each warp for itself: a barrier of all would have no limit if one of them gave up
+      if (lane == 0) mbar_arrive_cluster(leader_acc_empty + 8u * static_cast<uint32_t>(buf));
     }
   }
 
@@ -753,6 +753,12 @@ ltxq_status ltxq_qlinear_fp4(const ltxq_fp4_act* x, int64_t M, const ltxq_qweigh
   if (M < 0) return fail(LTXQ_ERR_INVALID, "qlinear_fp4: M < 0");
   if (!fp4::is_fp4(w->mode) || w->layout != LTXQ_LAYOUT_STD)
     return fail(LTXQ_ERR_UNSUPPORTED, "qlinear_fp4: the weight must be mxfp4 or nvfp4 in the standard layout");
+  float gx, gw;
+  if (ltxq_status st = fp4::check_act(x, M, w->k_in, &gx, "qlinear_fp4")) return st;
+  if (ltxq_status st = fp4_global_scale(w->mode, w->global_scale, &gw, "qlinear_fp4")) return st;
+  // one fp32 factor of the sums, with room for the 2^8 of decoded weights (fp4.cuh)
+  if (gx * gw < 0x1p-96f || gx * gw > 0x1p96f)
+    return fail(LTXQ_ERR_UNSUPPORTED, "qlinear_fp4: the product of the global scales must be within [2^-96, 2^96]");
   gemm::Params p{};
   if (ltxq_status st = qlinear_params(x->codes, M, *w, epi, out, &p)) return st;
   if (M == 0) return LTXQ_OK;

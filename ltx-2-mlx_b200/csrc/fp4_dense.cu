@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 2);
+      mbar_init(&acc_empty[b], 2 * kEpiWarps);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int m0, n0, sp, kb_lo, kb_hi;
       unit(u, m0, n0, sp, kb_lo, kb_hi);
       const int buf = it & 1;
-      if (!mbar_wait(&acc_full[buf], (it >> 1) & 1, abort_flag, p.err)) break;
+      if (!mbar_wait_warp(&acc_full[buf], (it >> 1) & 1, abort_flag, p.err)) break;
       tc_fence_after();
       const uint32_t tacc = tmem + t_lane + static_cast<uint32_t>(buf * BN);
       const int m0w = m0 + q * 32;  // first token of this warp
@@ -226,8 +226,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         gemm::epi_rows32(p, u8, m0w, n0 + c * 32, gated, two_round, gtab);
       }
       tc_fence_before();
-      gemm::named_bar_sync(1, 32 * kEpiWarps);
-      if (threadIdx.x == 0) mbar_arrive_cluster(leader_acc_empty + 8u * static_cast<uint32_t>(buf));
+      __syncwarp();  // each warp for itself: a barrier of all would have no limit if one of them gave up
+      if (lane == 0) mbar_arrive_cluster(leader_acc_empty + 8u * static_cast<uint32_t>(buf));
     }
   }
 

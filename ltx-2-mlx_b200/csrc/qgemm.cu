@@ -361,7 +361,7 @@ __device__ __forceinline__ void dequant_loop_fp4(const Params& p, const Bars& bb
     const uint32_t sc = s0;
     s0 = s1;
     s1 = scales(kb + 4);
-    if (!mbar_wait(&bb.w_full[s], (g / S) & 1, bb.abort_flag, p.err)) return;
+    if (!mbar_wait_warp(&bb.w_full[s], (g / S) & 1, bb.abort_flag, p.err)) return;
     // 32-byte rows, 32B swizzle: 16-byte chunk c sits at c ^ ((r >> 2) & 1)
     const uint8_t* wrow = ws + s * kWStage + r * QTraits<QK>::kWBytes;
     uint32_t o[32];
@@ -388,7 +388,7 @@ __device__ __forceinline__ void dequant_loop_fp4(const Params& p, const Bars& bb
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&bb.w_empty[s]);  // packed bytes consumed
-    if (!mbar_wait(&bb.a_empty[as], ((g / AS) & 1) ^ 1, bb.abort_flag, p.err)) return;
+    if (!mbar_wait_warp(&bb.a_empty[as], ((g / AS) & 1) ^ 1, bb.abort_flag, p.err)) return;
     const uint32_t dst = tmem + (static_cast<uint32_t>(q * 32) << 16) + kACol + as * 32;
     tmem_st_32x32b_x16(dst, o);
     tmem_st_32x32b_x16(dst + 16, o + 16);

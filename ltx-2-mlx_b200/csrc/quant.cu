@@ -243,8 +243,8 @@ ltxq_status ltxq_dequantize(const ltxq_qweight* w, void* out_bf16, void* stream)
     float g;
     if (ltxq_status st = fp4_global_scale(w->mode, w->global_scale, &g, "dequantize")) return st;
     if (R > 0x7FFFFFFF / 2 || L > 0x7FFFFFFF / 2) return fail(LTXQ_ERR_UNSUPPORTED, "dequantize: dimension too large");
-    if (reinterpret_cast<uintptr_t>(w->weight) & 15u)
-      return fail(LTXQ_ERR_UNSUPPORTED, "dequantize: the codes must be 16-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(w->weight) | reinterpret_cast<uintptr_t>(out_bf16)) & 15u)
+      return fail(LTXQ_ERR_UNSUPPORTED, "dequantize: the codes and the output must be 16-byte aligned");
     return launch_fp4_dequantize_rows(static_cast<const uint8_t*>(w->weight), static_cast<const uint8_t*>(w->scales), R,
                                       L, w->mode, g, static_cast<uint16_t*>(out_bf16), s);
   }

@@ -311,13 +311,13 @@ __global__ void __launch_bounds__(kThreads) rotary_heads_kernel(const Args a) {
     if (r + 1 < n) load();
     if (w.rot) {
       float2 ph[V], cs[V];
-      float most = 0.f;
+      bool near = true;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         ph[i] = pos[r * a.n_axes + ax[i]];
-        most = fmaxf(most, fabsf(ph[i].x * f[i].x));
+        near = near && fabsf(ph[i].x * f[i].x) < kFarTurns;  // not for NaN: 0 times a position past fp32's range
       }
-      if (most < kFarTurns) {  // NaN falls out of fmaxf and is NaN below too
+      if (near) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           float c1, s1;

@@ -83,7 +83,28 @@ class QuantizedLinear:
             self.in_features = in_features or packed_len
         if mode == "affine" and self.biases is None:
             raise ValueError("affine quantization needs biases")
+        if mode in FP4_MODES:
+            self._check_fp4()
         self.compute = "dequant"
+
+    def _check_fp4(self) -> None:
+        """The fp4 arrays fit the layer: what the kernels read lies inside them."""
+        rows, length = ((self.in_features, self.out_features) if self.pretransposed
+                        else (self.out_features, self.in_features))
+        if (self.bits, self.group_size) != (4, QUANT_DEFAULTS[self.mode][0]):
+            raise ValueError(f"{self.mode} has 4 bits and group_size {QUANT_DEFAULTS[self.mode][0]}")
+        for t, name, shape, size in ((self.weight, "weight", (rows, length // 8), 4),
+                                     (self.scales, "scales", (rows, length // self.group_size), 1),
+                                     (self.bias, "bias", (self.out_features,), 2)):
+            if t is None:
+                continue
+            if tuple(t.shape) != shape or t.element_size() != size or not t.is_contiguous():
+                raise ValueError(f"{self.mode} {name} must be a contiguous {shape} of {size}-byte elements, got "
+                                 f"{tuple(t.shape)} {t.dtype}")
+            if t.device != self.weight.device:
+                raise ValueError(f"{name} is on {t.device}, the weight on {self.weight.device}")
+        if length % self.group_size:
+            raise ValueError(f"{length} values do not divide into groups of {self.group_size}")
 
     def set_compute(self, compute: str) -> "QuantizedLinear":
         """Select how GEMMs over this weight compute (``COMPUTE``); the MX
@@ -281,7 +302,8 @@ class QuantizedLinear:
         an ``MXActivation`` of that many terms for the next GEMM.
 
         With compute "fp4" on an mxfp4 / nvfp4 weight, ``x`` is quantized to
-        the weight's format in the call, or comes as an ``FP4Tensor`` of it."""
+        the weight's format in the call (nvfp4: with global_scale 1, which
+        saturates past 6 * 448), or comes as an ``FP4Tensor`` of it."""
         if self.mode in FP4_MODES or isinstance(x, FP4Tensor):
             if mx_out:
                 raise ValueError("mx_out needs an MXActivation input (the block-scaled fp8 kernels)")
@@ -327,6 +349,7 @@ class QuantizedLinear:
         cached = getattr(self, "_q4", None)
         # the scale tensor is kept, so that its id names no other one
         if cached is None or cached[0] != key:
+            self._check_fp4()
             cached = (key, self.qweight(), self.scales)
             self._q4 = cached
         return cached[1]

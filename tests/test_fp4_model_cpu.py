@@ -36,3 +36,57 @@ def test_microbench_knows_the_formats():
     for name in ("mxfp4", "nvfp4", "mxfp4_fp4", "nvfp4_fp4"):
         mode, bits, compute = mb.MODES[name]
         assert quant_defaults(mode, None, None)[1] == bits and compute in COMPUTE
+
+
+def _layer(weight, scales, bias=None, mode="nvfp4", n=16, k=96, bits=4, group=16):
+    from ltxq.quantized_linear import QuantizedLinear
+
+    lin = object.__new__(QuantizedLinear)  # the constructor wants a GPU's tensors
+    lin.weight, lin.scales, lin.bias, lin.mode, lin.pretransposed = weight, scales, bias, mode, False
+    lin.out_features, lin.in_features, lin.bits, lin.group_size = n, k, bits, group
+    return lin
+
+
+def test_arrays_must_fit_the_layer():
+    w, s = torch.zeros(16, 12, dtype=torch.uint32), torch.zeros(16, 6, dtype=torch.uint8)
+    b = torch.zeros(16, dtype=torch.bfloat16)
+    _layer(w, s)._check_fp4()
+    _layer(w, s, b)._check_fp4()
+    _layer(w, s[:, :3].contiguous(), mode="mxfp4", group=32)._check_fp4()
+    for bad in (_layer(w, s[:, :5]), _layer(w, s[:, :5].contiguous()), _layer(w, s[:15]), _layer(w[:15], s),
+                _layer(w, s.short()), _layer(w.view(torch.uint8).view(16, 48), s), _layer(w, s, b[:8]),
+                _layer(w, s, b.float()), _layer(w, s, k=128), _layer(w, s, n=17), _layer(w, s, group=32),
+                _layer(w, s, bits=8), _layer(w, s, mode="mxfp4")):
+        with pytest.raises(ValueError):
+            bad._check_fp4()
+
+
+def _descriptors(mode, gw, gx, n=16, k=64):
+    from ltxq import _lib
+
+    group = 16 if mode == _lib.NVFP4 else 32
+    w = _lib.QWeight(0x1000, 0x2000, None, None, n, k, mode, 4, group, _lib.LAYOUT_STD, global_scale=gw)
+    return w, _lib.Fp4Act(0x3000, 0x4000, mode, gx)
+
+
+@pytest.mark.parametrize("gw,gx", [(2.0 ** 60, 2.0 ** 60), (2.0 ** -50, 2.0 ** -50)])
+def test_product_of_tensor_scales_is_bounded(gw, gx):
+    import ctypes
+
+    from ltxq import _lib
+
+    w, x = _descriptors(_lib.NVFP4, gw, gx)
+    lib = _lib.load()
+    assert lib.ltxq_qlinear_fp4(ctypes.byref(x), 1, ctypes.byref(w), None, 0x5000, None) == _lib.ERR_UNSUPPORTED
+    assert b"global scales" in lib.ltxq_last_error()
+
+
+def test_dequantize_wants_an_aligned_output():
+    import ctypes
+
+    from ltxq import _lib
+
+    w, _ = _descriptors(_lib.MXFP4, 1.0, 1.0)
+    lib = _lib.load()
+    assert lib.ltxq_dequantize(ctypes.byref(w), 0x5008, None) == _lib.ERR_UNSUPPORTED
+    assert b"aligned" in lib.ltxq_last_error()

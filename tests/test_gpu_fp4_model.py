@@ -155,3 +155,47 @@ def test_microbench_modes(cuda, capsys):
                      "1", "--graph"])
     row = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
     assert all(row[m]["ms"] > 0 for m in ("mxfp4", "nvfp4", "mxfp4_fp4", "nvfp4_fp4"))
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("compute", ["dequant", "fp4"])
+def test_long_feed_forward_runs_its_parts(cuda, mode, compute):
+    """Enough rows that the weight is dequantized once: the prologue's and the
+    feed-forward's workspaces hold that too."""
+    import ltxq
+
+    gen = _gen(9)
+    ff = ltxq.FeedForward.from_linear(_randn(gen, 2048, 256, std=0.05), None, _randn(gen, 2048, 2048, std=0.02), None,
+                                      mode=mode)
+    ff.project_in.set_compute(compute)
+    ff.project_out.set_compute(compute)
+    x = _randn(gen, 1, 1550, 256)
+    scale, shift = (torch.randn(1, 1, 256, generator=gen, device="cuda") * 0.1 for _ in range(2))
+    h = ltxq.adaln_modulate(x, scale, shift, 1e-6)
+    want = ff.project_in(h, gelu=True)
+    assert torch.equal(ff.project_in(x, adaln=(scale, shift, 1e-6), gelu=True), want)
+    assert torch.equal(ff(h), ff.project_out(want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("per_head", [False, True])
+def test_rotary_positions_past_fp32(cuda, dtype, per_head):
+    """Frequency 0 turns by nothing, wherever the token is."""
+    import ltxq
+
+    x = torch.randn(1, 3, 2, 64, device="cuda").to(dtype)
+    pos = torch.tensor([1e300, -1e39, 5.0], dtype=torch.float64, device="cuda")
+    freqs = torch.zeros(2, 32, dtype=torch.float64, device="cuda")
+    assert torch.equal(ltxq.rotary(x, pos, freqs if per_head else freqs[0], 2), x)
+
+
+def test_rotary_output_refusals(cuda):
+    import ltxq
+
+    x = torch.randn(2, 3, 64, device="cuda")
+    pos, freqs = torch.arange(3, device="cuda"), torch.ones(32, dtype=torch.float64, device="cuda")
+    with pytest.raises(ValueError, match="memory of its own"):
+        ltxq.rotary(x, pos, freqs, 1, out=x[:1].expand(2, 3, 64))
+    for scale in (float("nan"), float("inf"), 1e39):
+        with pytest.raises(ValueError, match="finite"):
+            ltxq.rotary(x, pos, freqs, 1, scale=scale)
