@@ -194,7 +194,22 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
-// The same for a whole warp: one answer for every lane, so that a wait that ran
+// Launches in a chain: a kernel launched with chained_attr() may start while the
+// one before it on the stream still runs, once all of that one's CTAs have
+// called chain_trigger(); it sets itself up and calls chain_wait() before it
+// reads what the first one writes (then complete).  Neither does anything in a
+// kernel that is not launched so.  The first of a chain is launched plainly, so
+// everything before it is complete.
+__device__ __forceinline__ void chain_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+inline cudaLaunchAttribute chained_attr() {
+  cudaLaunchAttribute a = {};
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  return a;
+}
+
+// mbar_wait for a whole warp: one answer for every lane, so that a wait that ran
 // out never leaves part of a warp in front of a warp-wide instruction.
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                                unsigned int* err) {

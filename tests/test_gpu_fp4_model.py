@@ -199,3 +199,38 @@ def test_rotary_output_refusals(cuda):
     for scale in (float("nan"), float("inf"), 1e39):
         with pytest.raises(ValueError, match="finite"):
             ltxq.rotary(x, pos, freqs, 1, scale=scale)
+
+
+@pytest.mark.parametrize("compute,m", [("fp4", 40), ("fp4", 700), ("dequant", 1600)])
+def test_calls_in_a_row_share_the_workspace(cuda, compute, m):
+    """Two launches per call, the second set up while the first still runs,
+    and the next call writes the same workspace: eager and as one graph, the
+    results are those of calls that were waited for."""
+    import ltxq
+
+    gen = _gen(11)
+    lins = [ltxq.QuantizedLinear.from_linear(_randn(gen, 2048, 512, std=0.05), mode="mxfp4").set_compute(compute)
+            for _ in range(2)]
+    xs = [_randn(gen, m, 512) for _ in range(6)]
+    want = []
+    for i, x in enumerate(xs):
+        want.append(lins[i % 2](x))
+        torch.cuda.synchronize()
+
+    def run():
+        return [lins[i % 2](x) for i, x in enumerate(xs)]
+
+    for _ in range(5):
+        for got, w in zip(run(), want):
+            assert torch.equal(got, w)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        outs = run()
+    for _ in range(5):
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
