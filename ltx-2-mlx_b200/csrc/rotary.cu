@@ -263,32 +263,10 @@ __global__ void __launch_bounds__(kThreads) rotary_heads_kernel(const Args a) {
   __shared__ float2 pos[kTableMax];  // [row][axis]
   const int64_t row0 = blockIdx.x * static_cast<int64_t>(a.rows_per_cta);
   const int n = static_cast<int>(min(static_cast<int64_t>(a.rows_per_cta), a.rows - row0));
-  for (int i = threadIdx.x; i < n * a.n_axes; i += kThreads) {
-    const int r = i / a.n_axes, ax = i - r * a.n_axes;
-    const int64_t row = row0 + r;
-    const int64_t b = row / a.tokens, t = row - b * a.tokens;
-    const double p = load_pos(a, b, t, ax);
-    pos[i] = split2(a.inverse ? -p : p);
-  }
-  __syncthreads();
-  const int u = blockIdx.y * kThreads + threadIdx.x;
-  if (u >= a.units) return;
-  const int h = u / a.all_units, c = u - h * a.all_units;
+  const int threads = static_cast<int>(blockDim.x), u = blockIdx.y * threads + threadIdx.x;
+  const bool live = u < a.units;
+  const int h = live ? u / a.all_units : 0, c = live ? u - h * a.all_units : 0;
   const Unit<V, kHalf> w(a, c);
-  float2 f[V];
-  int ax[V];
-  if (w.rot) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int k = h * a.half + c * V + i;
-      f[i] = split2(__ldg(a.freqs + k) * kInvTwoPi);
-      ax[i] = a.axis ? __ldg(a.axis + k) : 0;
-      if (static_cast<unsigned>(ax[i]) >= static_cast<unsigned>(a.n_axes)) {
-        f[i].x = NAN;
-        ax[i] = 0;
-      }
-    }
-  }
   const T* x = static_cast<const T*>(a.x) + h * a.xs[2];
   T* out = static_cast<T*>(a.out) + h * a.os[2];
   int64_t b = row0 / a.tokens, t = row0 - b * a.tokens;
@@ -298,7 +276,37 @@ __global__ void __launch_bounds__(kThreads) rotary_heads_kernel(const Args a) {
     p.load(xr + w.e0);
     if (w.second) q.load(xr + w.e1);
   };
-  load();
+  // the first row, the frequencies and the positions are read at once
+  if (live) load();
+  double fd[V];
+  int ax[V];
+  if (w.rot && live) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      fd[i] = __ldg(a.freqs + h * a.half + c * V + i);
+      ax[i] = a.axis ? __ldg(a.axis + h * a.half + c * V + i) : 0;
+    }
+  }
+  for (int i = threadIdx.x; i < n * a.n_axes; i += threads) {
+    const int r = i / a.n_axes, ax1 = i - r * a.n_axes;
+    const int64_t row = row0 + r;
+    const int64_t b1 = row / a.tokens, t1 = row - b1 * a.tokens;
+    const double p1 = load_pos(a, b1, t1, ax1);
+    pos[i] = split2(a.inverse ? -p1 : p1);
+  }
+  __syncthreads();
+  if (!live) return;
+  float2 f[V];
+  if (w.rot) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      f[i] = split2(fd[i] * kInvTwoPi);
+      if (static_cast<unsigned>(ax[i]) >= static_cast<unsigned>(a.n_axes)) {
+        f[i].x = NAN;
+        ax[i] = 0;
+      }
+    }
+  }
 #pragma unroll 1
   for (int r = 0; r < n; ++r) {
     T* orow = out + b * a.os[0] + t * a.os[1];
@@ -341,12 +349,12 @@ __global__ void __launch_bounds__(kThreads) rotary_heads_kernel(const Args a) {
 }
 
 template <typename T, int V>
-static void launch(const Args& a, bool half_layout, dim3 grid, cudaStream_t s) {
+static void launch(const Args& a, bool half_layout, dim3 grid, int threads, cudaStream_t s) {
   if (half_layout) {
-    if (a.per_head) rotary_heads_kernel<T, V, true><<<grid, kThreads, 0, s>>>(a);
+    if (a.per_head) rotary_heads_kernel<T, V, true><<<grid, threads, 0, s>>>(a);
     else rotary_shared_kernel<T, V, true><<<grid, kThreads, 0, s>>>(a);
   } else {
-    if (a.per_head) rotary_heads_kernel<T, V, false><<<grid, kThreads, 0, s>>>(a);
+    if (a.per_head) rotary_heads_kernel<T, V, false><<<grid, threads, 0, s>>>(a);
     else rotary_shared_kernel<T, V, false><<<grid, kThreads, 0, s>>>(a);
   }
 }
@@ -416,22 +424,27 @@ extern "C" ltxq_status ltxq_rotary(const ltxq_rotary_args* r, void* stream) {
   a.inverse = r->inverse ? 1 : 0;
   if (a.per_head && a.n_axes > kTableMax) return fail(LTXQ_ERR_UNSUPPORTED, "rotary: at most 2048 position axes");
   // Rows per CTA, within the table: shared frequencies, 1024 items of work (a few per thread, the table's cost spread
-  // over every head); a row of frequencies per head, 16 rows for a thread's registers.  Fewer where that would leave
-  // SMs idle.
+  // over every head), fewer where that would leave SMs idle.  A row of frequencies per head: as many threads as a row
+  // has units, and rows so that the SMs are filled once, with 512 threads of 16-byte units or 1024 of narrower ones: a
+  // CTA's start (frequencies, positions and first row, one trip to memory) is worth about ten rows.  9216 x 32 x 128
+  // took 37.8 us with 16 rows a CTA, 43.6 with 8, 35.0 with the 32 that fill the SMs; 4000 x 32 x 36, whose units are
+  // 4 bytes, 12.6 us with 1024 threads an SM, 19.3 with 512.
   int64_t per, gy;
+  int threads = kThreads;
   const int sms = num_sms();
   if (a.per_head) {
-    gy = (a.units + kThreads - 1) / kThreads;
-    per = 16;
-    if (per > kTableMax / a.n_axes) per = kTableMax / a.n_axes;
-    a.units_per_cta = kThreads;
+    if (a.units < kThreads) threads = (a.units + 31) / 32 * 32;
+    gy = (a.units + threads - 1) / threads;
+    per = kTableMax / a.n_axes;
+    a.units_per_cta = threads;
   } else {
     a.units_per_cta = a.units < 1024 ? a.units : 1024;
     gy = (a.units + a.units_per_cta - 1) / a.units_per_cta;
     per = 1024 / a.units_per_cta;
     if (a.half > 0 && per > kTableMax / a.half) per = kTableMax / a.half;
   }
-  const int64_t enough = (a.rows * gy + 4 * sms - 1) / (4 * sms);
+  const int64_t ctas = static_cast<int64_t>(sms) * (!a.per_head ? 4 : (V * es == 16 ? 512 : 1024) / threads);
+  const int64_t enough = (a.rows * gy + ctas - 1) / ctas;
   if (per > enough) per = enough;
   if (per < 1) per = 1;
   const int64_t gx = (a.rows + per - 1) / per;
@@ -441,13 +454,13 @@ extern "C" ltxq_status ltxq_rotary(const ltxq_rotary_args* r, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool hl = r->layout == LTXQ_ROTARY_HALF;
   if (es == 2) {
-    if (V == 8) launch<uint16_t, 8>(a, hl, grid, s);
-    else if (V == 2) launch<uint16_t, 2>(a, hl, grid, s);
-    else launch<uint16_t, 1>(a, hl, grid, s);
+    if (V == 8) launch<uint16_t, 8>(a, hl, grid, threads, s);
+    else if (V == 2) launch<uint16_t, 2>(a, hl, grid, threads, s);
+    else launch<uint16_t, 1>(a, hl, grid, threads, s);
   } else {
-    if (V == 4) launch<float, 4>(a, hl, grid, s);
-    else if (V == 2) launch<float, 2>(a, hl, grid, s);
-    else launch<float, 1>(a, hl, grid, s);
+    if (V == 4) launch<float, 4>(a, hl, grid, threads, s);
+    else if (V == 2) launch<float, 2>(a, hl, grid, threads, s);
+    else launch<float, 1>(a, hl, grid, threads, s);
   }
   return launch_check("rotary launch");
 }
