@@ -247,11 +247,12 @@ class QuantizedLinear:
         """bf16 weight: [out, in] (standard) or [in, out] (pretransposed)."""
         shape = (self.in_features, self.out_features) if self.pretransposed else (self.out_features, self.in_features)
         out = torch.empty(shape, dtype=torch.bfloat16, device=self.weight.device)
-        q = self.qweight()
         if self.mode in FP4_MODES:
+            q = self._qweight_base(0, None)  # reads the scales as they lie, not the packed ones
             with _on(self.weight):
                 _lib.check(_lib.load().ltxq_dequantize(ctypes.byref(q), out.data_ptr(), _stream()), "dequantize")
             return out
+        q = self.qweight()
         _lib.check(_lib.load().ltxq_dequantize(ctypes.byref(q), out.data_ptr(), _stream()), "dequantize")
         return out
 
@@ -343,14 +344,16 @@ class QuantizedLinear:
 
     def _qweight4(self) -> _lib.QWeight:
         """``qweight()`` of an fp4 weight, kept until one of its tensors or
-        settings changes."""
-        key = (self.weight.data_ptr(), self.scales.data_ptr(), id(self.scales), _version(self.scales),
+        settings changes.  The packed scales are brought up to date first:
+        their memory may have been packed for other scales since (by another
+        reader of this weight), which no pointer shows."""
+        packed = self._fp4_scales() if self.computes_fp4() else None
+        key = (self.weight.data_ptr(), self.scales.data_ptr(), packed.data_ptr() if packed is not None else 0,
                self.bias.data_ptr() if self.bias is not None else 0, self.compute, self.global_scale)
         cached = getattr(self, "_q4", None)
-        # the scale tensor is kept, so that its id names no other one
         if cached is None or cached[0] != key:
             self._check_fp4()
-            cached = (key, self.qweight(), self.scales)
+            cached = (key, self._qweight_base(0, packed.data_ptr() if packed is not None else None))
             self._q4 = cached
         return cached[1]
 

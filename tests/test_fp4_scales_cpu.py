@@ -1,0 +1,90 @@
+"""The packed scales of an fp4 weight and the descriptor that points at them,
+on the CPU: a fake library that copies scale bytes stands for the packing
+kernel, and the pointers of the descriptor are read as host memory."""
+
+import contextlib
+import ctypes
+
+import pytest
+import torch
+
+from ltxq import quantized_linear as Q
+
+
+class FakeLibrary:
+    """Packing is a copy, now or, where it is only recorded (``recording``), later."""
+
+    def __init__(self):
+        self.log, self.recording, self.recorded = [], False, []
+
+    def ltxq_fp4_weight_scales_size(self, q):
+        return self._q(q).n_out * self._q(q).k_in // 16
+
+    def ltxq_fp4_pack_weight_scales(self, q, out, stream):
+        self.log.append("pack")
+        job = (out, self._q(q).scales, self.ltxq_fp4_weight_scales_size(q))
+        if self.recording:
+            self.recorded.append(job)
+        else:
+            ctypes.memmove(*job)
+        return 0
+
+    def ltxq_dequantize(self, q, out, stream):
+        return 0
+
+    @staticmethod
+    def _q(q):
+        return getattr(q, "_obj", q)
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    fake = FakeLibrary()
+    monkeypatch.setattr(Q._lib, "load", lambda: fake)
+    monkeypatch.setattr(Q, "_on", lambda t: contextlib.nullcontext())
+    monkeypatch.setattr(Q, "_stream", lambda: 0)
+    monkeypatch.setattr(Q, "_capturing", lambda: fake.recording, raising=False)
+    monkeypatch.setattr(Q, "_wait_device", lambda dev: fake.log.append("device"), raising=False)
+    monkeypatch.setattr(Q, "_wait_stream", lambda: fake.log.append("stream"), raising=False)
+    return fake
+
+
+def _scales(fill, n=16, k=96):
+    return torch.full((n, k // 16), fill, dtype=torch.uint8)
+
+
+def _linear(n=16, k=96):
+    lin = object.__new__(Q.QuantizedLinear)  # the constructor wants a GPU's tensors
+    lin.weight, lin.scales = torch.zeros(n, k // 8, dtype=torch.uint32), _scales(1, n, k)
+    lin.biases = lin.bias = None
+    lin.mode, lin.pretransposed, lin.bits, lin.group_size = "nvfp4", False, 4, 16
+    lin.out_features, lin.in_features, lin.global_scale = n, k, 1.0
+    return lin.set_compute("fp4")
+
+
+def _read(q, n=16, k=96):
+    """The packed bytes a product with this descriptor reads: one value in these tests."""
+    got = set(ctypes.string_at(q.mx_scales, n * k // 16))
+    assert len(got) == 1
+    return got.pop()
+
+
+def test_descriptor_follows_what_other_readers_pack(lib):
+    """Scales swapped, packed by another reader, and swapped back."""
+    lin = _linear()
+    a, b = lin.scales, _scales(2)
+    for other in (lin.mx_scales, lin.qweight, lin.dequantize, lambda: lin.set_compute("fp4")):
+        assert _read(lin._qweight4()) == 1
+        lin.scales = b
+        other()
+        lin.scales = a
+        assert _read(lin._qweight4()) == 1
+        assert _read(lin.qweight()) == 1
+
+
+def test_reading_a_weight_back_packs_nothing(lib):
+    lin = _linear()
+    lin.scales = _scales(2)
+    del lib.log[:]
+    lin.dequantize()
+    assert "pack" not in lib.log

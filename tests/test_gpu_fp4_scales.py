@@ -1,0 +1,38 @@
+"""Scales of an fp4 weight that change between calls: the product always uses
+the ones the weight has, whoever packed them last.  Every comparison is of bits."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _weights(seed=21, n=128, k=256):
+    """A weight whose compute is "fp4", and one of twice its values: the same codes, other scales."""
+    from ltxq.quantized_linear import QuantizedLinear
+
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    w = torch.randn(n, k, generator=gen, device="cuda").bfloat16()
+    one, two = (QuantizedLinear.from_linear(v, mode="nvfp4").set_compute("fp4") for v in (w, w * 2))
+    assert torch.equal(one.weight, two.weight)
+    return one, two, gen
+
+
+@pytest.mark.parametrize("m", [3, 40, 700])
+def test_scales_swapped_back_after_another_reader_packed(cuda, m):
+    import ltxq
+
+    lin, twice, gen = _weights()
+    x = torch.randn(m, 256, generator=gen, device="cuda").bfloat16()
+    want, other = lin(x), twice(x)
+    ff = ltxq.FeedForward(lin, ltxq.QuantizedLinear.from_linear(torch.randn(64, 128, device="cuda").bfloat16(), mode="nvfp4"))
+    a, b = lin.scales, twice.scales.clone()
+    for reader in (lin.dequantize, lin.qweight, lin.mx_scales, lambda: ff(x), lambda: lin(x)):
+        lin.scales = b
+        reader()
+        lin.scales = a
+        assert torch.equal(lin(x), want)
+        lin.scales = b
+        assert torch.equal(lin(x), other)
+        lin.scales = a
+        assert torch.equal(lin(x), want)
