@@ -37,6 +37,11 @@ COMPUTE = {"dequant": _lib.COMPUTE_DEQUANT, "mx2": _lib.COMPUTE_MX2, "mx1": _lib
            "fp4": _lib.COMPUTE_FP4}
 
 
+def _capturing() -> bool:
+    """Whether the current stream records a graph."""
+    return torch.cuda.is_current_stream_capturing()
+
+
 def _version(t: torch.Tensor) -> int:
     """torch's in-place version counter (tensors made in inference mode have none)."""
     return 0 if t.is_inference() else t._version
@@ -116,9 +121,9 @@ class QuantizedLinear:
         self._mx_scales = None
         self._q4 = None
         if getattr(self, "_fp4_packed", None) is not None:
-            self._fp4_packed = (None, 0, self._fp4_packed[2])  # packed again, in place
+            self._fp4_packed = (None, None, self._fp4_packed[2])  # packed again, in place
         if compute != "dequant":
-            self.mx_scales()  # packed now, not inside a later stream capture
+            self.mx_scales()  # packed now, not in every replay of a later stream capture
         return self
 
     def mx_scales(self) -> torch.Tensor | None:
@@ -150,19 +155,26 @@ class QuantizedLinear:
         place, is packed again by the next call or ``set_compute``, into the
         same memory, which captured graphs read.  A graph replayed after such
         a change therefore needs one of the two first.  Tensors made in
-        inference mode do not count their changes, so ``set_compute`` always
-        packs."""
-        scales, version, buf = getattr(self, "_fp4_packed", (None, 0, None))
-        if scales is not self.scales or version != _version(self.scales):
+        inference mode do not count their changes, nor does ``.data`` of any
+        tensor, so ``set_compute`` always packs.
+
+        Inside a stream capture packing would only be recorded: memory of the
+        graph's own takes it there, packed by every replay, and nothing is
+        noted as packed."""
+        scales, state, buf = getattr(self, "_fp4_packed", (None, None, None))
+        now = (self.scales.data_ptr(), _version(self.scales))
+        if scales is not self.scales or state != now:
             with _on(self.scales):
                 lib = _lib.load()
                 q = self._qweight_base(0, None)
                 nbytes = lib.ltxq_fp4_weight_scales_size(ctypes.byref(q))
-                if buf is None or buf.numel() != nbytes or buf.device != self.scales.device:
+                recorded = _capturing()
+                if recorded or buf is None or buf.numel() != nbytes or buf.device != self.scales.device:
                     buf = torch.empty(nbytes, dtype=torch.uint8, device=self.scales.device)
                 _lib.check(lib.ltxq_fp4_pack_weight_scales(ctypes.byref(q), buf.data_ptr(), _stream()),
                            "fp4_pack_weight_scales")
-            self._fp4_packed = (self.scales, _version(self.scales), buf)
+            if not recorded:
+                self._fp4_packed = (self.scales, now, buf)
         return buf
 
     def computes_fp4(self) -> bool:
@@ -222,7 +234,9 @@ class QuantizedLinear:
 
     def qweight(self) -> _lib.QWeight:
         mx = self.mx_scales()
-        return self._qweight_base(self.data_flags(), mx.data_ptr() if mx is not None else None)
+        q = self._qweight_base(self.data_flags(), mx.data_ptr() if mx is not None else None)
+        q.packed = mx  # memory of a recorded packing belongs to this descriptor alone
+        return q
 
     def data_flags(self) -> int:
         """LTXQ_QW_* flags of the packed data (``ltxq_qweight_scan``), cached
@@ -353,8 +367,11 @@ class QuantizedLinear:
         cached = getattr(self, "_q4", None)
         if cached is None or cached[0] != key:
             self._check_fp4()
-            cached = (key, self._qweight_base(0, packed.data_ptr() if packed is not None else None))
-            self._q4 = cached
+            q = self._qweight_base(0, packed.data_ptr() if packed is not None else None)
+            q.packed = packed
+            cached = (key, q)
+            if packed is None or packed is getattr(self, "_fp4_packed", (None, None, None))[2]:
+                self._q4 = cached
         return cached[1]
 
     def _call_fp4(self, x, gelu, residual, gate, gate_then_add, adaln, split_k):

@@ -88,3 +88,47 @@ def test_reading_a_weight_back_packs_nothing(lib):
     del lib.log[:]
     lin.dequantize()
     assert "pack" not in lib.log
+
+
+def test_packing_that_is_only_recorded_counts_for_nothing_else(lib):
+    """In a capture the packing is part of the graph: a call outside before its
+    first replay packs for itself, and the graph leaves that memory alone."""
+    lin = _linear()
+    for change in ("in place", "replaced"):
+        before = lin.mx_scales()
+        if change == "in place":
+            lin.scales.fill_(5)
+        else:
+            lin.scales = _scales(6)
+        want = 5 if change == "in place" else 6
+        lib.recording = True
+        q = lin._qweight4()
+        assert lib.recorded and all(job[0] != before.data_ptr() for job in lib.recorded)
+        lib.recording = False
+        assert _read(lin._qweight4()) == want
+        assert lin.mx_scales() is before
+        for job in lib.recorded:  # the replay
+            ctypes.memmove(*job)
+        assert _read(q) == want and _read(lin._qweight4()) == want
+        del lib.recorded[:]
+
+
+def test_packed_before_a_capture_nothing_is_recorded(lib):
+    lin = _linear()
+    lin.mx_scales()
+    lib.recording = True
+    q = lin._qweight4()
+    assert not lib.recorded and _read(q) == 1
+
+
+def test_recorded_packing_keeps_its_memory_while_the_descriptor_lives(lib):
+    lin = _linear()
+    lin.scales = _scales(3)
+    del lin._fp4_packed  # never packed before
+    lib.recording = True
+    assert lin._qweight4().mx_scales
+    first, second = lin.qweight(), lin.qweight()
+    assert first.mx_scales != second.mx_scales
+    lin.set_compute("fp4")
+    lib.recording = False
+    assert _read(lin._qweight4()) == 3

@@ -36,3 +36,51 @@ def test_scales_swapped_back_after_another_reader_packed(cuda, m):
         assert torch.equal(lin(x), other)
         lin.scales = a
         assert torch.equal(lin(x), want)
+
+
+@pytest.mark.parametrize("change", ["in place", "replaced", "never packed"])
+def test_capture_before_any_call_sees_a_change(cuda, change):
+    """The packing goes into the graph; calls outside do not count on it, before the first replay or after."""
+    lin, twice, gen = _weights()
+    x = torch.randn(40, 256, generator=gen, device="cuda").bfloat16()
+    old, want = lin(x), twice(x)
+    if change == "in place":
+        lin.scales.copy_(twice.scales)
+    elif change == "replaced":
+        lin.scales = twice.scales.clone()
+    else:
+        lin, want = type(lin)(lin.weight, lin.scales, group_size=16, bits=4, mode="nvfp4"), old
+        lin.compute = "fp4"
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        out = lin(x)
+        second = lin(x)
+    assert torch.equal(lin(x), want)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(second, want) and torch.equal(lin(x), want)
+    if change == "in place":
+        lin.scales.fill_(0)
+        assert not lin(x).any()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert not out.any()
+
+
+def test_compute_set_inside_a_capture(cuda):
+    lin, twice, gen = _weights()
+    x = torch.randn(40, 256, generator=gen, device="cuda").bfloat16()
+    want = twice(x)
+    lin.scales.copy_(twice.scales)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        out = lin.set_compute("fp4")(x)
+    assert torch.equal(lin(x), want)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
