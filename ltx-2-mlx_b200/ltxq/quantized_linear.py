@@ -42,6 +42,14 @@ def _capturing() -> bool:
     return torch.cuda.is_current_stream_capturing()
 
 
+def _wait_device(device) -> None:
+    torch.cuda.synchronize(device)
+
+
+def _wait_stream() -> None:
+    torch.cuda.current_stream().synchronize()
+
+
 def _version(t: torch.Tensor) -> int:
     """torch's in-place version counter (tensors made in inference mode have none)."""
     return 0 if t.is_inference() else t._version
@@ -158,6 +166,10 @@ class QuantizedLinear:
         inference mode do not count their changes, nor does ``.data`` of any
         tensor, so ``set_compute`` always packs.
 
+        Calls on other streams cannot be told of a packing that they did not
+        ask for, so the host waits: for the device before memory is packed
+        again, which they may still read, and for the packing itself.
+
         Inside a stream capture packing would only be recorded: memory of the
         graph's own takes it there, packed by every replay, and nothing is
         noted as packed."""
@@ -171,8 +183,12 @@ class QuantizedLinear:
                 recorded = _capturing()
                 if recorded or buf is None or buf.numel() != nbytes or buf.device != self.scales.device:
                     buf = torch.empty(nbytes, dtype=torch.uint8, device=self.scales.device)
+                else:
+                    _wait_device(buf.device)
                 _lib.check(lib.ltxq_fp4_pack_weight_scales(ctypes.byref(q), buf.data_ptr(), _stream()),
                            "fp4_pack_weight_scales")
+                if not recorded:
+                    _wait_stream()
             if not recorded:
                 self._fp4_packed = (self.scales, now, buf)
         return buf

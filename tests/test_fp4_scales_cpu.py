@@ -132,3 +132,25 @@ def test_recorded_packing_keeps_its_memory_while_the_descriptor_lives(lib):
     lin.set_compute("fp4")
     lib.recording = False
     assert _read(lin._qweight4()) == 3
+
+
+def test_packing_is_ordered_against_every_stream(lib):
+    """Memory that other streams may still read is waited for before it is
+    packed again, and every packing is finished before a call on another
+    stream can find it; neither inside a capture."""
+    lin = _linear()
+    assert lib.log == ["pack", "stream"]  # memory of its own: nothing reads it yet
+    lin._qweight4(), lin.mx_scales()
+    assert lib.log == ["pack", "stream"]
+    del lib.log[:]
+    lin.scales.fill_(4)
+    lin._qweight4()
+    assert lib.log == ["device", "pack", "stream"]
+    del lib.log[:]
+    lin.set_compute("fp4")
+    assert lib.log == ["device", "pack", "stream"]
+    del lib.log[:]
+    lin.scales.fill_(5)
+    lib.recording = True
+    lin._qweight4()
+    assert lib.log == ["pack"]

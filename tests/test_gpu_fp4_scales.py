@@ -84,3 +84,34 @@ def test_compute_set_inside_a_capture(cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+def test_changed_scales_on_two_streams(cuda):
+    """Both streams wait for the change; the first call packs, behind a delay
+    of its stream, and the second finds the scales packed.  Then the other way
+    round: a delayed product still reads what the next change packs over."""
+    lin, twice, gen = _weights()
+    x = torch.randn(40, 256, generator=gen, device="cuda").bfloat16()
+    one, two = lin(x), twice(x)
+    sets = [lin.scales.clone(), twice.scales.clone()]
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(6):
+        want, scales = ((two, one)[i % 2], sets[1 - i % 2])
+        lin.scales.copy_(scales)
+        for s in (a, b):
+            s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(a):
+            torch.cuda._sleep(20_000_000)  # about 10 ms
+            first = lin(x)
+        with torch.cuda.stream(b):
+            second = lin(x)
+            torch.cuda._sleep(20_000_000)
+            third = lin(x)
+        torch.cuda.current_stream().wait_stream(a)  # the next change waits for a alone
+        lin.scales.copy_(sets[i % 2])
+        fourth = lin(x)
+        torch.cuda.synchronize()
+        for got in (first, second, third):
+            assert torch.equal(got, want)
+        assert torch.equal(fourth, (one, two)[i % 2])
