@@ -416,7 +416,7 @@ extern "C" ltxq_status ltxq_rotary(const ltxq_rotary_args* r, void* stream) {
   a.half = static_cast<int>(half);
   a.n_axes = r->n_axes;
   a.pos_type = r->pos_dtype;
-  a.per_head = r->freqs_per_head ? 1 : 0;
+  a.per_head = r->freqs_per_head && half > 0 ? 1 : 0;  // a copy reads no positions, which may be NULL
   a.rot_units = a.half / V;
   a.all_units = a.rot_units + (a.d - 2 * a.half + 2 * V - 1) / (2 * V);
   a.units = a.heads * a.all_units;
