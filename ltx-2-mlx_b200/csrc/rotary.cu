@@ -81,7 +81,8 @@ __device__ __forceinline__ void cos_sin_part(int q, float r, float& c, float& s)
 
 // cos and sin of t turns, any t: t = q / 4 + r, exact in fp64
 __device__ __noinline__ void cos_sin_far(double t, float& c, float& s) {
-  if (!(fabs(t) < 1e15)) t = t - rint(t);  // keeps 4t inside the adding trick's range; NaN and infinity give NaN
+  // the sum below stays in [2^52, 2^53), where its unit is 1, for |4t| < 2^51; NaN and infinity give NaN
+  if (!(fabs(t) < 0x1p49)) t = t - rint(t);
   constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
   const double m = __dadd_rn(4.0 * t, kRound);
   cos_sin_part(__double2loint(m), static_cast<float>(__fma_rn(__dsub_rn(m, kRound), -0.25, t)), c, s);

@@ -50,3 +50,26 @@ def test_no_frequencies_for_each_head(cuda, n_axes):
     axes = torch.zeros(3, 0, dtype=torch.int32, device="cuda")
     got = ltxq.rotary(x, p, f, 3, axes=axes) if n_axes > 1 else ltxq.rotary(x, p[:, 0], f, 3)
     assert torch.equal(got, x)
+
+
+@pytest.mark.parametrize("per_head", [False, True])
+def test_quadrants_of_far_positions(cuda, per_head):
+    """The fp64 value of pi / 2 times the kernel's 1 / (2 pi) is exactly a quarter turn, and a quarter times an integer
+    below 2^53 is exact: position n is turned by n quarters, whatever its size.  2^-21: an fp32 rotation."""
+    import math
+
+    import numpy as np
+
+    import ltxq
+
+    n = np.array([2 ** 51 + 1, 2 ** 51 - 1, 2400000000000001, 2400000000000003, -2400000000000001, -2400000000000002,
+                  -2 ** 51 - 3, 4000000000000001, -4000000000000001, 2 ** 53 - 1, 1 - 2 ** 53, 4 * 262144 + 3], np.int64)
+    assert (math.pi / 2) * 0.15915494309189535 == 0.25
+    x = torch.zeros(1, len(n), 8, device="cuda")
+    x[..., :4] = 1
+    f = torch.full((1, 4) if per_head else (4,), math.pi / 2, dtype=torch.float64, device="cuda")
+    for inverse in (False, True):
+        y = ltxq.rotary(x, torch.from_numpy(n).cuda(), f, 1, inverse=inverse).double().cpu().numpy()[0]
+        q = (-n if inverse else n) % 4
+        assert np.abs(y[:, 0] - np.array([1, 0, -1, 0])[q]).max() <= 2.0 ** -21
+        assert np.abs(y[:, 4] - np.array([0, 1, 0, -1])[q]).max() <= 2.0 ** -21
