@@ -257,7 +257,11 @@ ltxq_status ltxq_qk_norm_rope_pair(const void* q, const void* k, int64_t rows, i
  * forward call.  Angles are formed and reduced in two fp32 parts (in fp64 from
  * 2^20 turns on), the rotation is fp32, one rounding to the output type.  An
  * axis outside [0, n_axes) gives NaN.  With rotary_dim 0 the call copies, and
- * positions, freqs and axis are not read and may be NULL. */
+ * positions, freqs and axis are not read and may be NULL.  Elements of out are
+ * written in no order: out's strides give each its own place (every stride
+ * steps over all that smaller ones reach), and out is x with x's strides or
+ * shares no element with it; ranges that overlap are taken where both have the
+ * same strides. */
 enum { LTXQ_ROTARY_HALF = 0, LTXQ_ROTARY_INTERLEAVED = 1 };
 enum { LTXQ_POS_I32 = 0, LTXQ_POS_I64 = 1, LTXQ_POS_F32 = 2, LTXQ_POS_F64 = 3 };
 typedef struct {

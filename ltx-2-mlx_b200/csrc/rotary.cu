@@ -349,6 +349,74 @@ __global__ void __launch_bounds__(kThreads) rotary_heads_kernel(const Args a) {
   }
 }
 
+// ---------------------------------------------------------------- memory of x and out (host)
+
+using Wide = __int128;  // strides times sizes of any call
+
+// the axes of more than one element, by stride, smallest first (a head's elements among them)
+struct Axes {
+  int n = 0;
+  int64_t size[4];
+  Wide stride[4];
+  Wide reach[5];  // largest distance of two elements along the first i axes
+  Wide lo = 0, hi = 0;  // first and last element
+  Axes(const ltxq_rotary_args& r, const int64_t* s) {
+    const int64_t sz[4] = {r.head_dim, r.heads, r.tokens, r.batch}, st[4] = {1, s[2], s[1], s[0]};
+    for (int i = 0; i < 4; ++i) {
+      if (sz[i] <= 1) continue;
+      const Wide last = static_cast<Wide>(sz[i] - 1) * st[i];
+      (last < 0 ? lo : hi) += last;
+      int at = n++;
+      const Wide a = st[i] < 0 ? -static_cast<Wide>(st[i]) : st[i];
+      for (; at > 0 && stride[at - 1] > a; --at) {
+        size[at] = size[at - 1];
+        stride[at] = stride[at - 1];
+      }
+      size[at] = sz[i];
+      stride[at] = a;
+    }
+    reach[0] = 0;
+    for (int i = 0; i < n; ++i) reach[i + 1] = reach[i] + static_cast<Wide>(size[i] - 1) * stride[i];
+  }
+  // every stride steps over all that the smaller ones reach: no element is met twice
+  bool nested() const {
+    for (int i = 0; i < n; ++i)
+      if (stride[i] <= reach[i]) return false;
+    return true;
+  }
+  // nested axes: whether some two elements lie `delta` apart, by the first k axes
+  bool meets(Wide delta, int k) const {
+    if (k == 0) return delta == 0;
+    const Wide s = stride[k - 1];
+    Wide i = delta / s;  // or the next one down: what is left has to be within reach of the smaller axes
+    if (delta < 0 && i * s != delta) --i;
+    for (int c = 0; c < 2; ++c, ++i) {
+      const Wide rest = delta - i * s;
+      if (i > -size[k - 1] && i < size[k - 1] && rest <= reach[k - 1] && -rest <= reach[k - 1] && meets(rest, k - 1))
+        return true;
+    }
+    return false;
+  }
+};
+
+// Threads rotate their own elements with no order among them, so out has one
+// place for each, and shares one with x only as x itself.
+static ltxq_status check_memory(const ltxq_rotary_args& r, int es) {
+  const Axes x(r, r.x_stride), o(r, r.out_stride);
+  constexpr Wide kFar = static_cast<Wide>(1) << 60;
+  if (x.reach[x.n] >= kFar || o.reach[o.n] >= kFar) return fail(LTXQ_ERR_UNSUPPORTED, "rotary: strides too large");
+  if (!o.nested()) return fail(LTXQ_ERR_INVALID, "rotary: out must have memory of its own for every element");
+  const int64_t sizes[3] = {r.batch, r.tokens, r.heads};
+  bool same = true;  // of two layouts with the same strides it can be told whether they meet
+  for (int i = 0; i < 3; ++i) same = same && (sizes[i] <= 1 || r.x_stride[i] == r.out_stride[i]);
+  const Wide bytes = static_cast<Wide>(reinterpret_cast<uintptr_t>(r.out)) -
+                     static_cast<Wide>(reinterpret_cast<uintptr_t>(r.x));
+  if (same && bytes == 0) return LTXQ_OK;
+  if (bytes + o.lo * es >= (x.hi + 1) * es || bytes + (o.hi + 1) * es <= x.lo * es) return LTXQ_OK;  // apart
+  if (same && bytes % es == 0 && !o.meets(bytes / es, o.n)) return LTXQ_OK;
+  return fail(LTXQ_ERR_INVALID, "rotary: out must be x itself (with its strides) or share no memory with it");
+}
+
 template <typename T, int V>
 static void launch(const Args& a, bool half_layout, dim3 grid, int threads, cudaStream_t s) {
   if (half_layout) {
@@ -389,6 +457,7 @@ extern "C" ltxq_status ltxq_rotary(const ltxq_rotary_args* r, void* stream) {
   const int es = r->dtype == LTXQ_BF16 ? 2 : 4;
   if ((reinterpret_cast<uintptr_t>(r->x) | reinterpret_cast<uintptr_t>(r->out)) % es != 0)
     return fail(LTXQ_ERR_UNSUPPORTED, "rotary: x / out not aligned to their elements");
+  if (ltxq_status st = check_memory(*r, es)) return st;
 
   Args a{};
   a.x = r->x;

@@ -469,8 +469,10 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, heads:
     An axis outside [0, A) gives NaN.
 
     ``inverse`` turns back by the same angles with the same scale: the
-    gradient of the forward call.  ``out`` (x's shape and type) may be ``x``,
-    or share no element with it.
+    gradient of the forward call.  ``out`` (x's shape and type, memory of its
+    own for every element) may be ``x``, or share no element with it, which
+    has to show from the strides: two overlapping ranges of memory are taken
+    where both have the same ones.
     Returns ``out``, contiguous where it is made here."""
     _require_cuda(x, "x")
     _require_cuda(positions, "positions")
@@ -525,8 +527,6 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, heads:
         raise ValueError(f"scale must be finite, got {scale}")
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    elif out is not x and any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
-        raise ValueError("out must have memory of its own for every element")
     elif out.shape != x.shape or out.dtype != x.dtype or (out.stride(-1) != 1 and out.shape[-1] > 1):
         raise ValueError("out must have x's shape and type and a unit last stride")
     if x.numel() == 0:

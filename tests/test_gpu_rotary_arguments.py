@@ -73,3 +73,57 @@ def test_quadrants_of_far_positions(cuda, per_head):
         q = (-n if inverse else n) % 4
         assert np.abs(y[:, 0] - np.array([1, 0, -1, 0])[q]).max() <= 2.0 ** -21
         assert np.abs(y[:, 4] - np.array([0, 1, 0, -1])[q]).max() <= 2.0 ** -21
+
+
+def _freqs(n):
+    return 10000.0 ** (-torch.arange(n, dtype=torch.float64, device="cuda") / n)
+
+
+def test_outputs_beside_the_input(cuda):
+    """Everything that shares no element with x is written, whatever memory lies between."""
+    import ltxq
+
+    p, f = torch.arange(21, device="cuda"), _freqs(32)
+    buf = torch.randn(2, 21, 3, 4, 64, device="cuda").bfloat16()
+    rows = buf.view(2, 21, 768)
+    want = ltxq.rotary(rows[..., :256].clone(), p, f, 4)
+    for out in (rows[..., 256:512], rows[..., 512:]):  # columns of the same rows
+        before = rows.clone()
+        assert ltxq.rotary(rows[..., :256], p, f, 4, out=out) is out and torch.equal(out, want)
+        out.copy_(before[..., out.storage_offset() % 768:][..., :256])
+        assert torch.equal(rows, before)
+    flat = torch.zeros(4 * 2 * 21 * 256, device="cuda").bfloat16()
+    x = flat[:2 * 21 * 256].view(2, 21, 256)
+    x.copy_(rows[..., :256])
+    for i in (1, 3):  # behind one another
+        out = flat[i * 2 * 21 * 256:][:2 * 21 * 256].view(2, 21, 256)
+        assert torch.equal(ltxq.rotary(x, p, f, 4, out=out), want)
+    both = torch.zeros(2, 21, 8, 64, device="cuda").bfloat16()  # alternate heads
+    both[:, :, ::2] = rows[..., :256].view(2, 21, 4, 64)
+    ltxq.rotary(both[:, :, ::2], p, f, 4, out=both[:, :, 1::2])
+    assert torch.equal(both[:, :, 1::2].reshape(2, 21, 256), want)
+    turned = torch.zeros(2, 4, 21, 64, device="cuda").bfloat16().transpose(1, 2)
+    assert torch.equal(ltxq.rotary(rows[..., :256].view(2, 21, 4, 64), p, f, 4, out=turned).reshape(2, 21, 256), want)
+    view = x.view(2, 21, 256)  # another tensor object over x itself
+    assert torch.equal(ltxq.rotary(x, p, f, 4, out=view), want) and torch.equal(x, want)
+    one = torch.randn(1, 1, 256, device="cuda").bfloat16()
+    assert torch.equal(ltxq.rotary(one, p[:1], f, 4, out=one.expand(1, 1, 256)), one)
+
+
+def test_outputs_that_share_elements_are_refused(cuda):
+    import ltxq
+
+    p, f = torch.arange(3, device="cuda"), _freqs(32)
+    flat = torch.zeros(2000, device="cuda").bfloat16()
+    x = flat[:2 * 3 * 64].view(2, 3, 64)
+    for out in (flat[8:][:384].view(2, 3, 64), flat[64:][:384].view(2, 3, 64), flat[1:][:384].view(2, 3, 64),
+                flat.as_strided((2, 3, 64), (64, 128, 1))):
+        with pytest.raises(ValueError, match="x itself"):
+            ltxq.rotary(x, p, f, 1, out=out)
+    for rows in (flat[:64].expand(2, 3, 64), flat[:192].view(1, 3, 64).expand(2, 3, 64), flat.as_strided((2, 3, 64), (192, 32, 1))):
+        with pytest.raises(ValueError, match="memory of its own"):
+            ltxq.rotary(rows, p, f, 1, out=rows)
+        with pytest.raises(ValueError, match="memory of its own"):
+            ltxq.rotary(x.clone(), p, f, 1, out=rows)
+        assert torch.equal(ltxq.rotary(rows, p, f, 1), ltxq.rotary(rows.clone(), p, f, 1))  # read only: fine
+    assert not flat.any()
