@@ -457,6 +457,10 @@ extern "C" ltxq_status ltxq_rotary(const ltxq_rotary_args* r, void* stream) {
   const int es = r->dtype == LTXQ_BF16 ? 2 : 4;
   if ((reinterpret_cast<uintptr_t>(r->x) | reinterpret_cast<uintptr_t>(r->out)) % es != 0)
     return fail(LTXQ_ERR_UNSUPPORTED, "rotary: x / out not aligned to their elements");
+  const uintptr_t ps = r->pos_dtype == LTXQ_POS_I32 || r->pos_dtype == LTXQ_POS_F32 ? 4 : 8;
+  if (r->rotary_dim > 0 && (reinterpret_cast<uintptr_t>(r->positions) % ps != 0 ||
+                            reinterpret_cast<uintptr_t>(r->freqs) % 8 != 0 || reinterpret_cast<uintptr_t>(r->axis) % 4 != 0))
+    return fail(LTXQ_ERR_UNSUPPORTED, "rotary: positions, freqs and axis must be aligned to their elements");
   if (ltxq_status st = check_memory(*r, es)) return st;
 
   Args a{};

@@ -54,3 +54,11 @@ def test_out_that_overlaps_x(kw):
 def test_extents_past_64_bits():
     big = (1 << 62) - 8
     assert _status(batch=1 << 30, out_stride=(big, 128, 64), x_stride=(0, 128, 64))[0] in ("invalid", "unsupported")
+
+
+@pytest.mark.parametrize("kw", [dict(positions=20), dict(positions=18, pos_dtype=0), dict(positions=17, pos_dtype=2),
+                                dict(positions=20, pos_dtype=3), dict(freqs=20), dict(axis=18), dict(axis=17, n_axes=3),
+                                dict(freqs=12, freqs_per_head=1)])
+def test_unaligned_positions_and_frequencies(kw):
+    status, text = _status(**kw)
+    assert status == "unsupported" and "aligned to their elements" in text
