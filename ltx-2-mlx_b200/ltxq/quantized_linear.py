@@ -176,6 +176,7 @@ class QuantizedLinear:
         scales, state, buf = getattr(self, "_fp4_packed", (None, None, None))
         now = (self.scales.data_ptr(), _version(self.scales))
         if scales is not self.scales or state != now:
+            self._check_fp4()
             with _on(self.scales):
                 lib = _lib.load()
                 q = self._qweight_base(0, None)
@@ -249,10 +250,13 @@ class QuantizedLinear:
             COMPUTE[getattr(self, "compute", "dequant")], mx_scales, getattr(self, "global_scale", 1.0))
 
     def qweight(self) -> _lib.QWeight:
+        if self.mode in FP4_MODES:
+            kept = self._qweight4()
+            q = type(kept).from_buffer_copy(kept)
+            q.packed = kept.packed
+            return q
         mx = self.mx_scales()
-        q = self._qweight_base(self.data_flags(), mx.data_ptr() if mx is not None else None)
-        q.packed = mx  # memory of a recorded packing belongs to this descriptor alone
-        return q
+        return self._qweight_base(self.data_flags(), mx.data_ptr() if mx is not None else None)
 
     def data_flags(self) -> int:
         """LTXQ_QW_* flags of the packed data (``ltxq_qweight_scan``), cached
@@ -373,22 +377,31 @@ class QuantizedLinear:
         return out
 
     def _qweight4(self) -> _lib.QWeight:
-        """``qweight()`` of an fp4 weight, kept until one of its tensors or
-        settings changes.  The packed scales are brought up to date first:
-        their memory may have been packed for other scales since (by another
-        reader of this weight), which no pointer shows."""
+        """``qweight()`` of an fp4 weight, kept for its arrays and settings (the
+        objects, where they lie and their shapes: an address alone may be
+        another array's by now) and made and checked again for others.  The
+        packed scales are brought up to date first: their memory may have been
+        packed for other scales since (by another reader of this weight),
+        which no pointer shows."""
         packed = self._fp4_scales() if self.computes_fp4() else None
-        key = (self.weight.data_ptr(), self.scales.data_ptr(), packed.data_ptr() if packed is not None else 0,
-               self.bias.data_ptr() if self.bias is not None else 0, self.compute, self.global_scale)
+        w, s, b = self.weight, self.scales, self.bias
+        key = (w.data_ptr(), w.shape, s.data_ptr(), s.shape, packed.data_ptr() if packed is not None else 0,
+               (b.data_ptr(), b.shape) if b is not None else None, self.out_features, self.in_features, self.mode,
+               self.bits, self.group_size, self.pretransposed, self.compute, self.global_scale)
         cached = getattr(self, "_q4", None)
-        if cached is None or cached[0] != key:
+        if cached is None or cached[0] is not w or cached[1] is not s or cached[2] is not b or cached[3] != key:
             self._check_fp4()
             q = self._qweight_base(0, packed.data_ptr() if packed is not None else None)
-            q.packed = packed
-            cached = (key, q)
+            q.packed = packed  # memory of a recorded packing belongs to this descriptor alone
+            cached = (w, s, b, key, q)
             if packed is None or packed is getattr(self, "_fp4_packed", (None, None, None))[2]:
                 self._q4 = cached
-        return cached[1]
+        return cached[4]
+
+    def __getstate__(self):
+        """Copies make their own: the descriptor holds addresses, and memory for
+        packed scales belongs to one weight."""
+        return {k: v for k, v in self.__dict__.items() if k not in ("_q4", "_fp4_packed")}
 
     def _call_fp4(self, x, gelu, residual, gate, gate_then_add, adaln, split_k):
         """Products over an mxfp4 / nvfp4 weight, from bf16 rows or an ``FP4Tensor``."""

@@ -154,3 +154,68 @@ def test_packing_is_ordered_against_every_stream(lib):
     lib.recording = True
     lin._qweight4()
     assert lib.log == ["pack"]
+
+
+def _same_place(t, *shape, stride=None):
+    """Another array at t's address."""
+    return t.as_strided(shape, stride or torch.empty(shape, dtype=torch.uint8).stride())
+
+
+@pytest.mark.parametrize("name,other", [
+    ("weight", lambda lin: _same_place(lin.weight, 8, 12)), ("weight", lambda lin: _same_place(lin.weight, 16, 6)),
+    ("weight", lambda lin: _same_place(lin.weight, 16, 12, stride=(6, 1))),
+    ("weight", lambda lin: lin.weight.view(torch.uint8)), ("scales", lambda lin: _same_place(lin.scales, 8, 6)),
+    ("scales", lambda lin: _same_place(lin.scales, 16, 6, stride=(1, 1))),
+    ("bias", lambda lin: _same_place(lin.bias, 8)), ("bias", lambda lin: _same_place(lin.bias, 16, stride=(0,))),
+    ("bias", lambda lin: lin.bias.float()),
+])
+def test_array_at_the_same_address_is_checked(lib, name, other):
+    """A descriptor is kept for arrays, not for addresses: another array there is looked at anew."""
+    lin = _linear()
+    lin.set_compute("dequant")
+    lin.bias = torch.zeros(16, dtype=torch.bfloat16)
+    lin._qweight4()
+    setattr(lin, name, other(lin))
+    with pytest.raises(ValueError, match=name):
+        lin._qweight4()
+
+
+def test_layer_of_other_sizes_is_checked(lib):
+    for name, value in (("in_features", 192), ("out_features", 32), ("group_size", 32), ("bits", 8), ("mode", "mxfp4")):
+        lin = _linear()
+        lin.set_compute("dequant")
+        lin._qweight4()
+        setattr(lin, name, value)
+        with pytest.raises(ValueError):
+            lin._qweight4()
+
+
+def test_array_changed_under_its_object_is_checked(lib):
+    lin = _linear()
+    lin.set_compute("dequant")
+    lin._qweight4()
+    lin.weight.data = lin.weight[:8]
+    with pytest.raises(ValueError, match="weight"):
+        lin._qweight4()
+
+
+def test_scales_are_checked_before_they_are_packed(lib):
+    lin = _linear()
+    del lib.log[:]
+    for reader in (lin.mx_scales, lin.qweight, lin._qweight4, lambda: lin.set_compute("fp4")):
+        lin.scales = torch.zeros(16, 3, dtype=torch.uint8)
+        with pytest.raises(ValueError, match="scales"):
+            reader()
+    assert lib.log == []
+
+
+def test_copies_have_descriptors_and_packed_scales_of_their_own(lib):
+    import copy
+
+    lin = _linear()
+    lin._qweight4()
+    for other in (copy.deepcopy(lin), copy.copy(lin)):
+        assert _read(other._qweight4()) == 1
+        other.scales = _scales(9)
+        assert _read(other._qweight4()) == 9 and _read(lin._qweight4()) == 1
+        assert other._qweight4().weight == other.weight.data_ptr()
