@@ -65,6 +65,9 @@ def quant_defaults(mode: str, group_size: int | None, bits: int | None) -> tuple
 
 
 class QuantizedLinear:
+    _q4 = None  # the descriptor of an fp4 weight's products (_qweight4)
+    _fp4_packed = (None, None, None)  # scale tensor, its state, the memory its scales are packed in (_fp4_scales)
+
     def __init__(self, weight: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor | None = None,
                  bias: torch.Tensor | None = None, *, group_size: int, bits: int, mode: str = "affine",
                  pretransposed: bool = False, in_features: int | None = None, out_features: int | None = None,
@@ -128,8 +131,7 @@ class QuantizedLinear:
         self.compute = compute
         self._mx_scales = None
         self._q4 = None
-        if getattr(self, "_fp4_packed", None) is not None:
-            self._fp4_packed = (None, None, self._fp4_packed[2])  # packed again, in place
+        self._fp4_packed = (None, None, self._fp4_packed[2])  # packed again, in place
         if compute != "dequant":
             self.mx_scales()  # packed now, not in every replay of a later stream capture
         return self
@@ -173,7 +175,7 @@ class QuantizedLinear:
         Inside a stream capture packing would only be recorded: memory of the
         graph's own takes it there, packed by every replay, and nothing is
         noted as packed."""
-        scales, state, buf = getattr(self, "_fp4_packed", (None, None, None))
+        scales, state, buf = self._fp4_packed
         now = (self.scales.data_ptr(), _version(self.scales))
         if scales is not self.scales or state != now:
             self._check_fp4()
@@ -383,20 +385,25 @@ class QuantizedLinear:
         packed scales are brought up to date first: their memory may have been
         packed for other scales since (by another reader of this weight),
         which no pointer shows."""
-        packed = self._fp4_scales() if self.computes_fp4() else None
         w, s, b = self.weight, self.scales, self.bias
-        key = (w.data_ptr(), w.shape, s.data_ptr(), s.shape, packed.data_ptr() if packed is not None else 0,
-               (b.data_ptr(), b.shape) if b is not None else None, self.out_features, self.in_features, self.mode,
-               self.bits, self.group_size, self.pretransposed, self.compute, self.global_scale)
-        cached = getattr(self, "_q4", None)
-        if cached is None or cached[0] is not w or cached[1] is not s or cached[2] is not b or cached[3] != key:
-            self._check_fp4()
-            q = self._qweight_base(0, packed.data_ptr() if packed is not None else None)
-            q.packed = packed  # memory of a recorded packing belongs to this descriptor alone
-            cached = (w, s, b, key, q)
-            if packed is None or packed is getattr(self, "_fp4_packed", (None, None, None))[2]:
-                self._q4 = cached
-        return cached[4]
+        key = (w.data_ptr(), w.shape, s.data_ptr(), s.shape, (b.data_ptr(), b.shape) if b is not None else None,
+               self.out_features, self.in_features, self.mode, self.bits, self.group_size, self.pretransposed,
+               self.compute, self.global_scale)
+        kept = self._q4
+        if kept is not None and kept[0] is w and kept[1] is s and kept[2] is b and kept[3] == key:
+            q = kept[4]
+            if q.packed is None:
+                return q
+            scales, state, buf = self._fp4_packed
+            if scales is s and buf is q.packed and state == (key[2], _version(s)):
+                return q
+        self._check_fp4()
+        packed = self._fp4_scales() if self.computes_fp4() else None
+        q = self._qweight_base(0, packed.data_ptr() if packed is not None else None)
+        q.packed = packed  # memory of a recorded packing belongs to this descriptor alone
+        if packed is None or packed is self._fp4_packed[2]:
+            self._q4 = (w, s, b, key, q)
+        return q
 
     def __getstate__(self):
         """Copies make their own: the descriptor holds addresses, and memory for
