@@ -21,8 +21,14 @@ from . import _lib
 _DT = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 
 
-_device = torch._C._cuda_getDevice  # the current device and its current stream, without wrapping objects
-_raw_stream = torch._C._cuda_getCurrentRawStream
+def _public_raw_stream(device: int) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+# The current device and a device's current stream: torch's own functions where it has them (built with CUDA; a
+# microsecond or two less per call), else the public ones.
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _public_raw_stream)
 
 
 def _stream() -> int:
