@@ -301,6 +301,12 @@ ltxq_status ltxq_qweight_scan(const ltxq_qweight* w, uint32_t* flags_out, void* 
 size_t ltxq_qlinear_workspace_size(int64_t M, const ltxq_qweight* w);
 size_t ltxq_adaln_qlinear_workspace_size(int64_t M, const ltxq_qweight* w);
 size_t ltxq_feed_forward_workspace_size(int64_t M, const ltxq_qweight* w_in, const ltxq_qweight* w_out);
+/* The part of ltxq_qlinear_workspace_size() without split-K partials: with it
+ * the same kernels run, every tile whole.  mxfp4 / nvfp4 weights with many rows
+ * (from 768 rows and 48 tiles of 256 x 256 on) are dequantized once into their
+ * workspace, 2 N K bytes of it; given less, the fused kernels convert the
+ * weight again for each 256 rows. */
+size_t ltxq_qlinear_unsplit_workspace_size(int64_t M, const ltxq_qweight* w);
 
 /* out[M, N] = epilogue(x[M, K] . dequant(W)^T); x, out bf16 row-major
  * (row strides K and N). */

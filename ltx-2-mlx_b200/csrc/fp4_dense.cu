@@ -280,9 +280,10 @@ static ltxq_status launch(const void* x, const void* w, const gemm::Params& p, c
 
 }  // namespace dense
 
-// Workspace of the dequantized weight (then of the split tiles' partial sums),
-// or 0 where the fused kernel runs.
-size_t fp4_dense_bytes(int64_t M, const ltxq_qweight& w, size_t* partial_offset) {
+// Workspace of the dequantized weight and behind it of the split tiles' partial
+// sums (from *weight_bytes on; without them no tile is split), or 0 where the
+// fused kernel runs.
+size_t fp4_dense_bytes(int64_t M, const ltxq_qweight& w, size_t* weight_bytes) {
   if ((w.mode != LTXQ_MXFP4 && w.mode != LTXQ_NVFP4) || w.layout != LTXQ_LAYOUT_STD || w.compute == LTXQ_COMPUTE_FP4)
     return 0;
   if (w.n_out <= 0 || w.k_in <= 0 || w.k_in % 32 != 0) return 0;
@@ -292,20 +293,22 @@ size_t fp4_dense_bytes(int64_t M, const ltxq_qweight& w, size_t* partial_offset)
   // 16384: 109 against 108, 1024 rows: 129 against 126)
   if (M < 768 || (M + 255) / 256 * ((w.n_out + 255) / 256) < 48) return 0;
   const size_t weight = (static_cast<size_t>(w.n_out) * static_cast<size_t>(w.k_in) * 2 + 255) & ~size_t(255);
-  if (partial_offset) *partial_offset = weight;
+  if (weight_bytes) *weight_bytes = weight;
   return weight + gemm::splitk_bytes(M, w.n_out, w.k_in);
 }
 
-// p as qlinear_params filled it, checked; workspace of fp4_dense_bytes(), 256-byte aligned.
+// p as qlinear_params filled it, checked; workspace 256-byte aligned, of fp4_dense_bytes()
+// or at least of their part for the weight.
 ltxq_status launch_qlinear_fp4_dense(const void* x, const ltxq_qweight& w, gemm::Params p, void* workspace,
-                                     cudaStream_t stream) {
+                                     size_t workspace_bytes, cudaStream_t stream) {
   if (ltxq_status st = launch_fp4_dequantize_rows(static_cast<const uint8_t*>(w.weight),
                                                   static_cast<const uint8_t*>(w.scales), w.n_out, w.k_in, w.mode, 1.f,
                                                   static_cast<uint16_t*>(workspace), stream))
     return st;
   size_t off = 0;
-  fp4_dense_bytes(p.M, w, &off);
-  const gemm::Sched sc = gemm::plan_schedule(p.M, p.N, p.K);
+  const size_t all = fp4_dense_bytes(p.M, w, &off);
+  gemm::Sched sc = gemm::plan_schedule(p.M, p.N, p.K);
+  if (workspace_bytes < all) sc.dp = sc.tiles, sc.splits = 1;
   p.dp_tiles = sc.dp;
   p.splits = sc.splits;
   p.partial = sc.splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(workspace) + off) : nullptr;

@@ -47,9 +47,9 @@ ltxq_status launch_qlinear_mx(const void* x, int64_t M, const ltxq_qweight& w, c
                               cudaStream_t stream);
 size_t fp4_workspace_bytes(int64_t M, const ltxq_qweight& w);
 bool fp4_rows_supported(int64_t M, const ltxq_qweight& w);
-size_t fp4_dense_bytes(int64_t M, const ltxq_qweight& w, size_t* partial_offset);
+size_t fp4_dense_bytes(int64_t M, const ltxq_qweight& w, size_t* weight_bytes);
 ltxq_status launch_qlinear_fp4_dense(const void* x, const ltxq_qweight& w, gemm::Params p, void* workspace,
-                                     cudaStream_t stream);
+                                     size_t workspace_bytes, cudaStream_t stream);
 ltxq_status launch_fp4_rows(const void* x, bool quantize, const ltxq_fp4_act* packed, const ltxq_qweight& w,
                             const gemm::Params& p, cudaStream_t stream);
 ltxq_status launch_qlinear_fp4_from_bf16(const void* x, int64_t M, const ltxq_qweight& w, const gemm::Params& p,
@@ -1623,9 +1623,10 @@ ltxq_status launch_qlinear(const void* x, int64_t M, const ltxq_qweight& w, cons
   }
 
   // many rows with an fp4 weight: dequantized once into the workspace
-  if (const size_t bytes = fp4_dense_bytes(M, w, nullptr)) {
-    if (workspace && workspace_bytes >= bytes && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0)
-      return launch_qlinear_fp4_dense(x, w, p, workspace, stream);
+  size_t weight_bytes = 0;
+  if (fp4_dense_bytes(M, w, &weight_bytes)) {
+    if (workspace && workspace_bytes >= weight_bytes && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0)
+      return launch_qlinear_fp4_dense(x, w, p, workspace, workspace_bytes, stream);
   }
 
   // native block-scaled fp8 path (LTXQ_COMPUTE_MX*), when it applies and the
@@ -1721,6 +1722,15 @@ size_t ltxq_qlinear_workspace_size(int64_t M, const ltxq_qweight* w) {
     if (const size_t d = ltxq::fp4_dense_bytes(M, *w, nullptr)) return ltxq::align_up(d);
   }
   return ltxq::align_up(ltxq::gemm::splitk_bytes(M, w->n_out, w->k_in));
+}
+
+size_t ltxq_qlinear_unsplit_workspace_size(int64_t M, const ltxq_qweight* w) {
+  if (!w || M <= 0) return 0;
+  if (const size_t mx = ltxq::mx_workspace_bytes(M, *w)) return ltxq::align_up(mx);
+  if (const size_t f4 = ltxq::fp4_workspace_bytes(M, *w)) return ltxq::align_up(f4);
+  size_t weight_bytes = 0;
+  if (ltxq::fp4_rows_supported(M, *w) || !ltxq::fp4_dense_bytes(M, *w, &weight_bytes)) return 0;
+  return ltxq::align_up(weight_bytes);
 }
 
 // With block-scaled weights (and the AdaLN pass able to write MX terms:

@@ -145,6 +145,7 @@ SIGNATURES = {
     "ltxq_quantize": (c_int32, [c_void_p, POINTER(QWeight), c_void_p]),
     "ltxq_dequantize": (c_int32, [POINTER(QWeight), c_void_p, c_void_p]),
     "ltxq_qlinear_workspace_size": (c_size_t, [c_int64, POINTER(QWeight)]),
+    "ltxq_qlinear_unsplit_workspace_size": (c_size_t, [c_int64, POINTER(QWeight)]),
     "ltxq_adaln_qlinear_workspace_size": (c_size_t, [c_int64, POINTER(QWeight)]),
     "ltxq_feed_forward_workspace_size": (c_size_t, [c_int64, POINTER(QWeight), POINTER(QWeight)]),
     "ltxq_qlinear": (c_int32, [c_void_p, c_int64, POINTER(QWeight), POINTER(Epilogue), c_void_p, c_void_p,

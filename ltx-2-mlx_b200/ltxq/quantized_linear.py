@@ -340,7 +340,10 @@ class QuantizedLinear:
 
         With compute "fp4" on an mxfp4 / nvfp4 weight, ``x`` is quantized to
         the weight's format in the call (nvfp4: with global_scale 1, which
-        saturates past 6 * 448), or comes as an ``FP4Tensor`` of it."""
+        saturates past 6 * 448), or comes as an ``FP4Tensor`` of it.  Many rows
+        over such a weight otherwise (from 768 rows and 48 tiles of 256 x 256
+        outputs on) take a workspace of the dequantized weight, 2 bytes per
+        value (134 MB at 4096 x 16384), besides that of split-K partials."""
         if self.mode in FP4_MODES or isinstance(x, FP4Tensor):
             if mx_out:
                 raise ValueError("mx_out needs an MXActivation input (the block-scaled fp8 kernels)")
@@ -457,7 +460,7 @@ class QuantizedLinear:
             pro = prologue(norm, adaln[2], adaln[0], adaln[1], tuple(rows_shape), self.in_features, keep)
             ws_bytes = lib.ltxq_adaln_qlinear_workspace_size(M, q)
         else:
-            ws_bytes = lib.ltxq_qlinear_workspace_size(M, q) if split_k or self.compute == "fp4" else 0
+            ws_bytes = (lib.ltxq_qlinear_workspace_size if split_k else lib.ltxq_qlinear_unsplit_workspace_size)(M, q)
         ws = out.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
         ws_ptr = ws.data_ptr() if ws is not None else None
         if pro is not None:

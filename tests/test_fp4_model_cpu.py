@@ -90,3 +90,24 @@ def test_dequantize_wants_an_aligned_output():
     lib = _lib.load()
     assert lib.ltxq_dequantize(ctypes.byref(w), 0x5008, None) == _lib.ERR_UNSUPPORTED
     assert b"aligned" in lib.ltxq_last_error()
+
+
+def test_unsplit_workspace():
+    """The part of the workspace that a product needs to run the same kernels unsplit."""
+    import ctypes
+
+    from ltxq import _lib
+
+    lib = _lib.load()
+    for mode in (_lib.MXFP4, _lib.NVFP4):
+        w, _ = _descriptors(mode, 1.0, 1.0, n=5120, k=544)
+        q = ctypes.byref(w)
+        both = lambda m: (lib.ltxq_qlinear_unsplit_workspace_size(m, q), lib.ltxq_qlinear_workspace_size(m, q))  # noqa: E731
+        assert both(0) == (0, 0) and both(16) == (0, 0)
+        assert both(200)[0] == 0  # the fused kernels
+        assert both(767)[0] == 0
+        assert both(768)[0] == 5120 * 544 * 2 <= both(768)[1]
+        w.compute, w.mx_scales = _lib.COMPUTE_FP4, 0x6000
+        assert both(200)[0] == both(200)[1] > 0 and both(2000)[0] == both(2000)[1] > both(200)[0]
+        assert both(16) == (0, 0)
+    assert lib.ltxq_qlinear_unsplit_workspace_size(4, None) == 0
