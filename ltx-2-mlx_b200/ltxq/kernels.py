@@ -203,11 +203,21 @@ class FP4Tensor:
                 self.buffer[self._scale_off:self._scale_off + self._scale_bytes])
 
     def struct(self) -> _lib.Fp4Act:
-        st = self._st
-        if st is None:
-            base = self.buffer.data_ptr()
-            st = self._st = _lib.Fp4Act(base, base + self._scale_off, FP4_MODES[self.mode], self.global_scale)
-        return st
+        base = self.buffer.data_ptr()
+        kept = self._st
+        if kept is None or kept[0] is not self.buffer or kept[1] != (base, self.mode, self.global_scale):
+            buf = self.buffer
+            if (buf.dtype != torch.uint8 or not buf.is_contiguous() or buf.numel() < self._scale_off + self._scale_bytes
+                    or base % 16):
+                raise ValueError("the buffer of an FP4Tensor holds its codes and scales: uint8, contiguous, 16-byte "
+                                 f"aligned, {self._scale_off + self._scale_bytes} bytes")
+            st = _lib.Fp4Act(base, base + self._scale_off, FP4_MODES[self.mode], self.global_scale)
+            kept = self._st = (buf, (base, self.mode, self.global_scale), st)
+        return kept[2]
+
+    def __getstate__(self):
+        """Copies make a descriptor of their own: it holds addresses."""
+        return self.__dict__ | {"_st": None}
 
     @classmethod
     def quantize(cls, x: torch.Tensor, mode: str = "nvfp4", global_scale: float = 1.0) -> "FP4Tensor":

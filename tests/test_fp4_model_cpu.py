@@ -111,3 +111,27 @@ def test_unsplit_workspace():
         assert both(200)[0] == both(200)[1] > 0 and both(2000)[0] == both(2000)[1] > both(200)[0]
         assert both(16) == (0, 0)
     assert lib.ltxq_qlinear_unsplit_workspace_size(4, None) == 0
+
+
+def test_quantized_tensor_describes_what_it_holds():
+    import copy
+
+    import ltxq
+
+    t = ltxq.FP4Tensor((3, 5), 288, "nvfp4", "cpu", 0.5)
+    st = t.struct()
+    codes, scales = t.tensors()
+    assert (st.codes, st.scales, st.global_scale) == (codes.data_ptr(), scales.data_ptr(), 0.5)
+    t.buffer = t.buffer.clone()
+    codes, scales = t.tensors()
+    st = t.struct()
+    assert (st.codes, st.scales) == (codes.data_ptr(), scales.data_ptr())
+    t.global_scale = 0.25
+    assert t.struct().global_scale == 0.25
+    other = copy.deepcopy(t)
+    st = other.struct()
+    assert st.codes == other.buffer.data_ptr() != t.buffer.data_ptr()
+    for bad in (t.buffer[:-1], t.buffer[1:], t.buffer[::2], t.buffer.view(torch.int16)):
+        other.buffer = bad
+        with pytest.raises(ValueError, match="buffer"):
+            other.struct()
