@@ -435,6 +435,11 @@ class QuantizedLinear:
             raise ValueError(f"x is on {device}, the weight on {self.weight.device}")
         if x.shape[-1] != self.in_features:
             raise ValueError(f"x last dim {x.shape[-1]} != in_features {self.in_features}")
+        if residual is not None or adaln is not None:
+            for t in (residual, gate, *(adaln[:2] if adaln is not None else ())):
+                if hasattr(t, "get_device") and t.get_device() != dev:  # what is no tensor is refused below
+                    raise ValueError(f"residual, gate, scale and shift must be on the weight's device "
+                                     f"({self.weight.device}), got {t.device}")
         if dev != _device():
             with torch.cuda.device(dev):
                 return self._call_fp4(x, gelu, residual, gate, gate_then_add, adaln, split_k)

@@ -135,3 +135,27 @@ def test_quantized_tensor_describes_what_it_holds():
         other.buffer = bad
         with pytest.raises(ValueError, match="buffer"):
             other.struct()
+
+
+def test_operands_on_another_device_are_refused(monkeypatch):
+    """A product's residual, gate and prologue vectors lie on its own device (stand-ins for tensors of two GPUs)."""
+    from ltxq import quantized_linear as Q
+
+    class On(SimpleNamespace):
+        def get_device(self):
+            return self.device.index
+
+        def new_empty(self, *a, **k):
+            return self
+
+    def on(i, *shape):
+        return On(device=torch.device("cuda", i), shape=shape, dtype=torch.bfloat16, numel=lambda: 4 * 96, is_cuda=True)
+
+    monkeypatch.setattr(Q, "_require_cuda", lambda t, name: None)
+    monkeypatch.setattr(Q, "_device", lambda: 0)
+    lin = _layer(on(0, 16, 12), None)
+    lin.compute = "dequant"
+    for kw in (dict(residual=on(1, 4, 16), gate=on(0, 16)), dict(residual=on(0, 4, 16), gate=on(1, 16)),
+               dict(adaln=(on(1, 96), on(0, 96), 1e-6)), dict(adaln=(on(0, 96), on(1, 96), 1e-6))):
+        with pytest.raises(ValueError, match="cuda:1"):
+            lin(on(0, 4, 96), **kw)
