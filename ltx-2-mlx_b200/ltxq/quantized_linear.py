@@ -28,6 +28,9 @@ from .kernels import (FP4_MODES, FP4Tensor, MXActivation, _device, _on, _raw_str
 
 QUANT_DEFAULTS = {"affine": (64, 4), "mxfp8": (32, 8), "mxfp4": (32, 4), "nvfp4": (16, 4)}
 _MODE = {"affine": _lib.AFFINE, "mxfp8": _lib.MXFP8, **FP4_MODES}
+# the types that an fp4 weight's scales come in: their bytes, or the format itself
+_SCALES = {"mxfp4": (torch.uint8, torch.int8, torch.float8_e8m0fnu),
+           "nvfp4": (torch.uint8, torch.int8, torch.float8_e4m3fn)}
 # how the GEMM computes (include/ltxq.h LTXQ_COMPUTE_*): "dequant" (bf16
 # tensor cores over the exactly dequantized weight), "mx2" / "mx1" (native
 # block-scaled fp8 MMAs on mxfp8 weights, activations in two / one MXFP8 terms),
@@ -109,13 +112,13 @@ class QuantizedLinear:
                         else (self.out_features, self.in_features))
         if (self.bits, self.group_size) != (4, QUANT_DEFAULTS[self.mode][0]):
             raise ValueError(f"{self.mode} has 4 bits and group_size {QUANT_DEFAULTS[self.mode][0]}")
-        for t, name, shape, size in ((self.weight, "weight", (rows, length // 8), 4),
-                                     (self.scales, "scales", (rows, length // self.group_size), 1),
-                                     (self.bias, "bias", (self.out_features,), 2)):
+        for t, name, shape, types in ((self.weight, "weight", (rows, length // 8), (torch.uint32, torch.int32)),
+                                      (self.scales, "scales", (rows, length // self.group_size), _SCALES[self.mode]),
+                                      (self.bias, "bias", (self.out_features,), (torch.bfloat16,))):
             if t is None:
                 continue
-            if tuple(t.shape) != shape or t.element_size() != size or not t.is_contiguous():
-                raise ValueError(f"{self.mode} {name} must be a contiguous {shape} of {size}-byte elements, got "
+            if tuple(t.shape) != shape or t.dtype not in types or not t.is_contiguous():
+                raise ValueError(f"{self.mode} {name} must be a contiguous {shape} of one of {types}, got "
                                  f"{tuple(t.shape)} {t.dtype}")
             if t.device != self.weight.device:
                 raise ValueError(f"{name} is on {t.device}, the weight on {self.weight.device}")

@@ -159,3 +159,17 @@ def test_operands_on_another_device_are_refused(monkeypatch):
                dict(adaln=(on(1, 96), on(0, 96), 1e-6)), dict(adaln=(on(0, 96), on(1, 96), 1e-6))):
         with pytest.raises(ValueError, match="cuda:1"):
             lin(on(0, 4, 96), **kw)
+
+
+def test_arrays_of_another_type_of_the_same_size_are_refused():
+    w, s = torch.zeros(16, 12, dtype=torch.uint32), torch.zeros(16, 6, dtype=torch.uint8)
+    b = torch.zeros(16, dtype=torch.bfloat16)
+    s32 = s[:, :3].contiguous()
+    for ok in (_layer(w.view(torch.int32), s, b), _layer(w, s.view(torch.float8_e4m3fn)), _layer(w, s.view(torch.int8)),
+               _layer(w, s32.view(torch.float8_e8m0fnu), mode="mxfp4", group=32)):
+        ok._check_fp4()
+    for bad in (_layer(w, s, b.half()), _layer(w, s, b.view(torch.int16)), _layer(w.view(torch.float32), s),
+                _layer(w, s.view(torch.float8_e5m2)), _layer(w, s.view(torch.float8_e8m0fnu)), _layer(w, s.bool()),
+                _layer(w, s32.view(torch.float8_e4m3fn), mode="mxfp4", group=32)):
+        with pytest.raises(ValueError, match="must be"):
+            bad._check_fp4()
