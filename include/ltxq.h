@@ -116,8 +116,8 @@ enum { LTXQ_COMPUTE_DEQUANT = 0, LTXQ_COMPUTE_MX2 = 1, LTXQ_COMPUTE_MX1 = 2, LTX
  *  mxfp8:   weight uint32 [N, K/4] (E4M3), scales uint8 E8M0 [N, K/32]
  *  mxfp4:   weight uint32 [N, K/8] (E2M1, low nibble first), scales uint8 E8M0
  *           [N, K/32]: w = code * 2^(scale - 127)
- *  nvfp4:   weight as mxfp4, scales uint8 E4M3 [N, K/16]:
- *           w = code * scale * global_scale
+ *  nvfp4:   weight as mxfp4, scales uint8 E4M3 [N, K/16], the sign bit clear
+ *           (COMPUTE_FP4 has no signed scales): w = code * scale * global_scale
  *  A NaN scale (0xFF E8M0, 0x7F E4M3) makes its whole group NaN; the
  *  quantizer writes it for a group that holds an infinity or a NaN, which
  *  E2M1 has no code for.

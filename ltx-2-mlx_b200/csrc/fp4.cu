@@ -15,7 +15,6 @@
 namespace ltxq {
 
 ltxq_status check_qweight(const ltxq_qweight& w, bool need_data, int64_t* R, int64_t* L);
-ltxq_status check_epilogue(const ltxq_epilogue* epi, int64_t M, int64_t N);
 bool fp4_rows_supported(int64_t M, const ltxq_qweight& w);
 ltxq_status launch_fp4_rows(const void* x, bool quantize, const ltxq_fp4_act* packed, const ltxq_qweight& w,
                             const gemm::Params& p, cudaStream_t stream);
@@ -215,7 +214,7 @@ namespace fp4 {
 // one per quarter, move them there through registers (tcgen05.st), one stage
 // ahead in the other of two buffers, while the MMAs of a stage run.  Copying
 // them with tcgen05.cp from the MMA's thread instead takes the tensor pipe's
-// own time, 54 cycles an atom: at 9216 x 16384 x 4096 nvfp4 the MMAs alone took
+// own time: at 9216 x 16384 x 4096 nvfp4 the MMAs alone took
 // 213 us, the copies alone 190 more, and the kernel 414.
 constexpr int BM = 128;       // tokens per block and CTA (MMA M = 256 for the pair)
 constexpr int BKB = kStageK / 2;  // bytes of one operand row in a stage

@@ -16,14 +16,17 @@
 // of a block (16 bytes each, streaming loads; the MMA's K order is a permutation
 // that x is laid out in too) and loads kT blocks ahead.
 //
-// Decoding bounds the kernel: 17 cycles per warp and word of 8 on a quarter of
-// an SM (integer pipe), 4 us of the 17 that one token through 4096 x 16384
-// takes; the rest is the first trip through the code (a launch runs each
-// instruction a few times only), x and the partial sums.  Measured and not
-// kept: the weight through shared memory, by cp.async or TMA, with the loops
-// rolled (17.7 to 20.8 us), and fp16 products, whose decoding the hardware does
-// at 7 cycles a word but whose x needs a scan of its range (17.7 us, 26 against
-// 18 at 8 rows).
+// One token through 4096 x 16384 (nvfp4) takes 17.3 us, 2.2 TB/s of weight.  No
+// unit is full: the counters of a launch from cold caches show the integer pipe,
+// on which the words are decoded, busy 36 % of the cycles and issue slots 38 %;
+// of a warp's time 41 % goes to waiting for its loads, 11 % to the barriers
+// around x and the partial sums, 11 % to the full pipe and 2 % to instructions
+// that are not there yet.  So the loads and the decoding, 16 warps of an SM in
+// step, overlap only in part.  Measured and not kept: the weight through shared
+// memory, by cp.async or TMA, with the loops rolled (17.7 to 20.8 us), and fp16
+// products, whose decoding takes the hardware half the cycles (11 per warp and
+// word of 8 on a quarter of an SM, against 23) but whose x needs a scan of its
+// range (17.7 us, 26 against 18 at 8 rows).
 #include "common.cuh"
 #include "fp4.cuh"
 #include "gemm_epilogue.cuh"

@@ -19,9 +19,13 @@
 // Memory-bound where the heads share the frequencies: the angles of a CTA's
 // rows are computed once into shared memory, and its threads walk (row, unit)
 // items, a unit being V neighbouring pairs of one head, two vectors of 16 bytes.
-// With a row of frequencies per head every pair has its own angle (about 40
-// instructions); a thread keeps one unit's frequencies in registers and walks
-// rows, loading the next one's x ahead.
+// With a row of frequencies per head every pair has its own angle (37
+// instructions, all told); a thread keeps one unit's frequencies in registers and
+// walks rows, loading the next one's x ahead.  Issue slots are busy 64 % of the
+// cycles there (1 x 9216 x 32 x 128 bf16, three axes: 35.6 us, 4.2 TB/s), and
+// with 110 registers 16 warps of an SM are all there are to fill the rest while
+// a quarter of their time goes to waiting for x: 512 threads have one row of 32
+// bytes each under way, 16 KB an SM.
 #include "common.cuh"
 
 namespace ltxq {
@@ -99,9 +103,10 @@ __device__ __forceinline__ float2 split2(double v) {
 constexpr float kFarTurns = 1048576.0f;
 
 // cos and sin of p * f turns, both as two parts, |p * f| < kFarTurns.  kShort:
-// for results that are rounded to bf16, the hardware's functions (off by at most
-// 2^-20.9 within a turn, where bf16 rounds by 2^-9 of a value): with them the
-// video grid's case is bound by memory, with the series by instructions.
+// for results that are rounded to bf16, by 2^-9 to 2^-8 of a value, the hardware's
+// functions, off by at most 2^-20.9 of the pair's length within a turn.  The
+// series costs about twice as much per pair: 9216 x 32 x 64 fp32, half the pairs
+// and the same bytes, takes 33.3 us where 9216 x 32 x 128 bf16 takes 35.
 template <bool kShort>
 __device__ __forceinline__ void cos_sin(float2 p, float2 f, float& c, float& s) {
   const float t = __fmul_rn(p.x, f.x);
