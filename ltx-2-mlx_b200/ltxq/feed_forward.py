@@ -16,7 +16,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .kernels import _require_cuda, _stream, prologue, vec_arg
+from .kernels import _device, _require_cuda, _stream, prologue, vec_arg
 from .quantized_linear import QuantizedLinear
 
 
@@ -50,6 +50,13 @@ class FeedForward:
             raise ValueError("x must be bfloat16")
         if x.shape[-1] != self.dim:
             raise ValueError(f"x last dim {x.shape[-1]} != {self.dim}")
+        dev = x.get_device()
+        for t in (self.project_in.weight, self.project_out.weight, gate, *(adaln[:2] if adaln is not None else ())):
+            if hasattr(t, "get_device") and t.get_device() != dev:  # what is no tensor is refused below
+                raise ValueError(f"weights, gate, scale and shift must be on x's device ({x.device}), got {t.device}")
+        if dev != _device():
+            with torch.cuda.device(dev):
+                return self._run(x, adaln, gate)
         x = x.contiguous()
         rows_shape = tuple(x.shape[:-1])
         M = x.numel() // self.dim
