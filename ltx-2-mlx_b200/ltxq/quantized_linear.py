@@ -287,6 +287,7 @@ class QuantizedLinear:
         shape = (self.in_features, self.out_features) if self.pretransposed else (self.out_features, self.in_features)
         out = torch.empty(shape, dtype=torch.bfloat16, device=self.weight.device)
         if self.mode in FP4_MODES:
+            self._check_fp4()
             q = self._qweight_base(0, None)  # reads the scales as they lie, not the packed ones
             with _on(self.weight):
                 _lib.check(_lib.load().ltxq_dequantize(ctypes.byref(q), out.data_ptr(), _stream()), "dequantize")

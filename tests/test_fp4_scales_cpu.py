@@ -219,3 +219,10 @@ def test_copies_have_descriptors_and_packed_scales_of_their_own(lib):
         other.scales = _scales(9)
         assert _read(other._qweight4()) == 9 and _read(lin._qweight4()) == 1
         assert other._qweight4().weight == other.weight.data_ptr()
+
+
+def test_arrays_are_checked_before_they_are_read_back(lib):
+    lin = _linear()
+    lin.scales = torch.zeros(16, 3, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="scales"):
+        lin.dequantize()
