@@ -168,8 +168,9 @@ class QuantizedLinear:
         place, is packed again by the next call or ``set_compute``, into the
         same memory, which captured graphs read.  A graph replayed after such
         a change therefore needs one of the two first.  Tensors made in
-        inference mode do not count their changes, nor does ``.data`` of any
-        tensor, so ``set_compute`` always packs.
+        inference mode do not count their changes, and writes through ``.data``,
+        by a replayed graph or from outside torch count for none: after those
+        call ``set_compute``, which always packs.
 
         Calls on other streams cannot be told of a packing that they did not
         ask for, so the host waits: for the device before memory is packed
