@@ -115,3 +115,43 @@ def test_changed_scales_on_two_streams(cuda):
         for got in (first, second, third):
             assert torch.equal(got, want)
         assert torch.equal(fourth, (one, two)[i % 2])
+
+
+@pytest.mark.parametrize("m", [40, 300])
+def test_feed_forward_captured_before_any_call_sees_a_change(cuda, m):
+    """Its descriptors keep the graph's own packed scales until the launch, beside a workspace of the same pool."""
+    import ltxq
+
+    def pair():
+        one, two, gen = _weights(n=512)
+        out1, out2, _ = _weights(seed=22, n=256, k=512)
+        return ltxq.FeedForward(one, out1), ltxq.FeedForward(two, out2), gen
+
+    ff, want_ff, gen = pair()
+    x = torch.randn(m, 256, generator=gen, device="cuda").bfloat16()
+    want, old = want_ff(x), ff(x)
+    ff.project_in.scales.copy_(want_ff.project_in.scales)
+    ff.project_out.scales = want_ff.project_out.scales.clone()
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        out = ff(x)
+    assert torch.equal(ff(x), want) and not torch.equal(old, want)
+    for _ in range(2):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_copies_keep_their_scales_apart(cuda):
+    import copy
+
+    lin, twice, gen = _weights()
+    x = torch.randn(40, 256, generator=gen, device="cuda").bfloat16()
+    one, two = lin(x), twice(x)
+    for other in (copy.copy(lin), copy.deepcopy(lin)):
+        assert torch.equal(other(x), one)
+        other.scales = twice.scales.clone()
+        assert torch.equal(other(x), two) and torch.equal(lin(x), one)
